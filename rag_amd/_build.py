@@ -22,6 +22,9 @@ HEADERS = ["common.h", "kernels.h", "encoder_ffn3.h", "encoder_qkv_attn.h", os.p
 # -ffp-contract=off: the canonical score is an explicit fmaf chain; nothing else may be fused.
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
          "-fhip-fp32-correctly-rounded-divide-sqrt", "-Wall", "-Wno-unused-function",
+         # no packed fp32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results on gfx950 now and
+         # then; hipcc makes them by itself from float2 and scalar code.  (Its host pass warns that it does not know the feature.)
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
          # the SGPR-base LDS-DMA helpers write M0 inside their asm and list it as clobbered (it is a reserved register)
          "-Wno-inline-asm"]
 
