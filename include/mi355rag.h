@@ -62,7 +62,7 @@ typedef enum {
 } mi_status;
 
 enum { MI_METRIC_IP = 0, MI_METRIC_L2 = 1 };
-enum { MI_DTYPE_F32 = 0, MI_DTYPE_BF16 = 1 };
+enum { MI_DTYPE_F32 = 0, MI_DTYPE_BF16 = 1, MI_DTYPE_F16 = 2 };   /* F16: mi_attention_* only */
 
 /* search path selection (mi_index_set_mode) */
 enum {
@@ -298,6 +298,69 @@ int  mi_encoder_encode_dev_noalloc(mi_encoder* enc, int64_t B, int L, const int3
                                    const int32_t* mask_dev, float* out_emb_dev, void* stream);
 /* Timing of the last encode pass (all kernels), HIP events on its stream. */
 int  mi_encoder_last_time(const mi_encoder* enc, float* out_ms);
+
+/* ------------------------------------------------------------------ packed attention
+ * Attention over whole sequences as an operator of its own, forward and backward, for the layers of embedding and reranking
+ * models: packed sequences of different lengths or a padded batch under a key mask, causal or not, grouped key / value heads,
+ * and a relative position bias learned by buckets.  No counterpart in the reference (its models run inside
+ * sentence-transformers, advanced_rag.py:104-107); the encoder calls it for models that are causal or carry such a bias
+ * (mi_encoder_set_attention).
+ *
+ *   s_ij = scale * q_i . k_j + bias_table[bucket(j - i)][head],  p = softmax over the attended j,  out_i = sum_j p_ij v_j
+ *
+ * over rows i, j of one sequence; j is attended when it is a key (key_mask, if given, is not 0 there) and, with `causal`,
+ * j <= i.  Query head h reads key head h / (heads / kv_heads).  A row that attends nothing has out = 0 and lse = -inf.
+ *
+ * A finite bias counts as at most 4096 in size; -inf takes its bucket's keys out.
+ *
+ * bucket(r), the scheme of relative-position encoders: bidirectional: n = num_buckets / 2, d = |r|, and n is added for r > 0;
+ * otherwise n = num_buckets, d = max(-r, 0).  With m = n / 2 the distances d < m have a bucket each, then
+ * m + floor((n - m) log(d / m) / log(max_distance / m)), at most n - 1; borders that are whole numbers are exact.
+ *
+ * Tensors are given as rows of head_dim 16-bit elements: row (token t, head h) starts at ptr + t * token_stride +
+ * h * head_stride (elements), its elements are adjacent.  ptr is 16-byte aligned, the strides are multiples of 8, head_dim is
+ * a multiple of 8 up to 128.  Sequence i is rows offsets[i] .. offsets[i + 1] (device int32 [nseq + 1], rising from 0, at most
+ * `tokens`; offsets outside that order give unspecified rows but no access outside the tensors); offsets = NULL: nseq
+ * sequences of tokens / nseq rows each.  Sequences may be empty.  Rows behind the last sequence are left as they were, or, with
+ * zero_tail, set to 0 (lse: -inf).  Values of one sequence never reach another, and rows that key_mask takes out may hold
+ * anything in k and v; a NaN or infinity in a row reaches the rows of its own sequence that attend it, and with `causal` may also
+ * reach earlier rows of that sequence.
+ * Softmax statistics and sums are fp32; p (and, backward, ds) is rounded to the tensors' type for the matrix product. */
+typedef struct {
+    int32_t heads, kv_heads;          /* heads a multiple of kv_heads */
+    int32_t head_dim;
+    int32_t dtype;                    /* MI_DTYPE_BF16 or MI_DTYPE_F16 */
+    int32_t causal;
+    int32_t zero_tail;
+    float   scale;                    /* > 0 */
+    int32_t num_buckets;              /* 0: no bias; else 2 (bidirectional: 4, even) .. 64 */
+    int32_t max_distance;             /* above the exact buckets' distances, at most 1024 */
+    int32_t bidirectional;
+} mi_attention_config;
+typedef struct {
+    const void* ptr;
+    int64_t token_stride, head_stride;
+} mi_attention_rows;
+/* lse: fp32 [heads][tokens], or NULL; the backward pass needs it.  bias_table: fp32 [num_buckets][heads] (NULL iff
+ * num_buckets is 0).  out may be the same rows as q (in place), and overlaps nothing else. */
+int  mi_attention_dev(mi_ctx* ctx, const mi_attention_config* cfg, int64_t tokens, int64_t nseq,
+                      const int32_t* offsets_dev, const int32_t* key_mask_dev, const mi_attention_rows* q,
+                      const mi_attention_rows* k, const mi_attention_rows* v, const float* bias_table_dev,
+                      const mi_attention_rows* out, float* lse_dev, void* stream);
+/* bucket(r) for n relative positions r = key - query (host arrays, no GPU call). */
+int  mi_attention_buckets(int num_buckets, int max_distance, int bidirectional, int64_t n, const int64_t* rel, int32_t* out);
+/* Gradients of sum(dout * out): dq, dk, dv (rows as above; dk and dv are the sums over a group's query heads), and, with a
+ * bias, dbias_table fp32 [num_buckets][heads] (overwritten, not added to).  out and lse are the forward pass's.  The results of
+ * a repeated call are the same bits: nothing is summed by atomics in an order of its own.  workspace_dev: 256-byte aligned,
+ * mi_attention_backward_workspace bytes (packed: offsets are given), the caller's alone until the work on the stream is done.
+ * dq, dk, dv overlap no input. */
+int  mi_attention_backward_workspace(const mi_attention_config* cfg, int64_t tokens, int64_t nseq, int packed, size_t* bytes);
+int  mi_attention_backward_dev(mi_ctx* ctx, const mi_attention_config* cfg, int64_t tokens, int64_t nseq,
+                               const int32_t* offsets_dev, const int32_t* key_mask_dev, const mi_attention_rows* q,
+                               const mi_attention_rows* k, const mi_attention_rows* v, const float* bias_table_dev,
+                               const mi_attention_rows* out, const float* lse_dev, const mi_attention_rows* dout,
+                               const mi_attention_rows* dq, const mi_attention_rows* dk, const mi_attention_rows* dv,
+                               float* dbias_table_dev, void* workspace_dev, size_t workspace_bytes, void* stream);
 
 /* ---- host text path: WordPiece tokenizer (pure host code, no GPU call)
  * Replaces the tokenizer advanced_rag.py:104-107 reaches through HuggingFaceEmbeddings ->

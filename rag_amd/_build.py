@@ -16,8 +16,8 @@ LIBDIR = os.path.join(HERE, "lib")
 OBJDIR = os.path.join(HERE, "..", "build", "obj")
 LIB = os.path.join(LIBDIR, "libmi355rag.so")
 
-SOURCES = ["capi.hip", "multi.hip", "ingest.hip", "search_exact.hip", "search_mfma.hip", "encoder.hip", "encoder_ffn3.hip", "encoder_qkv_attn.hip", "wordpiece.hip"]
-HEADERS = ["common.h", "kernels.h", "encoder_ffn3.h", "encoder_qkv_attn.h", os.path.join("..", "..", "include", "mi355rag.h")]
+SOURCES = ["capi.hip", "multi.hip", "ingest.hip", "search_exact.hip", "search_mfma.hip", "encoder.hip", "encoder_ffn3.hip", "encoder_qkv_attn.hip", "attention.hip", "wordpiece.hip"]
+HEADERS = ["common.h", "kernels.h", "encoder_ffn3.h", "encoder_qkv_attn.h", "attention.h", os.path.join("..", "..", "include", "mi355rag.h")]
 
 # -ffp-contract=off: the canonical score is an explicit fmaf chain; nothing else may be fused.
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",

@@ -16,7 +16,7 @@ LIB_PATH = os.environ.get("MI355RAG_LIB") or os.path.join(_HERE, "lib", "libmi35
 
 MI_OK = 0
 METRIC_IP, METRIC_L2 = 0, 1
-DTYPE_F32, DTYPE_BF16 = 0, 1
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 MODE_AUTO, MODE_EXACT, MODE_FAST = 0, 1, 2
 MAX_K = 2048
 
@@ -39,10 +39,23 @@ class BertConfig(ctypes.Structure):
                 ("normalize", ctypes.c_int32)]
 
 
+class AttentionConfig(ctypes.Structure):
+    """mi_attention_config"""
+    _fields_ = [("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("causal", ctypes.c_int32), ("zero_tail", ctypes.c_int32), ("scale", ctypes.c_float),
+                ("num_buckets", ctypes.c_int32), ("max_distance", ctypes.c_int32), ("bidirectional", ctypes.c_int32)]
+
+
+class AttentionRows(ctypes.Structure):
+    """mi_attention_rows"""
+    _fields_ = [("ptr", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
 # every symbol include/mi355rag.h declares: name -> (restype, argtypes)
 _vp, _i64, _i32, _u64 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_uint64
 _pp = ctypes.POINTER(ctypes.c_void_p)
 _cfgp = ctypes.POINTER(BertConfig)
+_acfgp, _rowsp = ctypes.POINTER(AttentionConfig), ctypes.POINTER(AttentionRows)
 SYMBOLS = {
     "mi_init": (_i32, [_i32, _pp]),
     "mi_ctx_destroy": (None, [_vp]),
@@ -107,6 +120,11 @@ SYMBOLS = {
     "mi_encoder_classify_ragged": (_i32, [_vp, _i64, _vp, _vp, _vp, _i32, _vp]),
     "mi_encoder_stats": (_i32, [_vp, ctypes.POINTER(ctypes.c_int64)]),
     "mi_encoder_last_time": (_i32, [_vp, ctypes.POINTER(ctypes.c_float)]),
+    "mi_attention_dev": (_i32, [_vp, _acfgp, _i64, _i64, _vp, _vp, _rowsp, _rowsp, _rowsp, _vp, _rowsp, _vp, _vp]),
+    "mi_attention_buckets": (_i32, [_i32, _i32, _i32, _i64, _vp, _vp]),
+    "mi_attention_backward_workspace": (_i32, [_acfgp, _i64, _i64, _i32, ctypes.POINTER(ctypes.c_size_t)]),
+    "mi_attention_backward_dev": (_i32, [_vp, _acfgp, _i64, _i64, _vp, _vp, _rowsp, _rowsp, _rowsp, _vp, _rowsp, _vp, _rowsp, _rowsp, _rowsp, _rowsp,
+                                         _vp, _vp, ctypes.c_size_t, _vp]),
     "mi_wordpiece_create": (_i32, [ctypes.c_char_p, _i64, _i32, _pp]),
     "mi_wordpiece_set_unicode": (_i32, [_vp, _i64, _vp, _vp, ctypes.c_char_p, _i64]),
     "mi_wordpiece_destroy": (None, [_vp]),
