@@ -20,6 +20,8 @@ struct mi_attn_args {
     const float* table = nullptr;         // [buckets][heads], or NULL
     float* delta = nullptr;               // backward workspace [heads][tokens]: rowsum(dout * out)
     float* partial = nullptr;             // backward workspace [heads][dq tiles][64]: the table gradient's block sums
+    float* parts_kv = nullptr;            // backward workspace [splits][dk | dv][tokens][key heads][hd], where splits > 1
+    int splits = 1;                       // shares of a group's query heads in the dK / dV kernel
     float* dtable = nullptr;              // [buckets][heads]
     int64_t tokens = 0;
     int nseq = 0, uniform_len = 0;
@@ -39,6 +41,6 @@ int mi_attn_buckets(const char* who, mi_attn_args* a, int buckets, int max_dista
 // The forward pass on device pointers (arguments already checked).
 int mi_launch_attention(hipStream_t st, mi_attn_args a, int dtype);
 
-// Bytes of workspace of the backward pass (fields offsets, tokens, nseq, uniform_len, heads, table, buckets), and the pass itself.
+// Bytes of workspace of the backward pass (fields offsets, tokens, nseq, uniform_len, heads, group, hd, table, buckets), and the pass itself.
 size_t mi_attn_backward_bytes(const mi_attn_args& a);
 int mi_launch_attention_backward(hipStream_t st, mi_attn_args a, int dtype, void* workspace);

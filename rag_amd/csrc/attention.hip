@@ -57,11 +57,6 @@ template <bool F16> __device__ __forceinline__ float at_hi(uint32_t w)
     if constexpr (F16) return (float)__builtin_bit_cast(f16x2, w)[1];
     else return __builtin_bit_cast(float, w & 0xFFFF0000u);
 }
-// *a += x in LDS, nothing returned; used only where one lane owns the address, so the order of the additions is the program's
-__device__ __forceinline__ void at_lds_add(float* a, float x)
-{
-    __builtin_amdgcn_ds_atomic_fadd_f32((__attribute__((address_space(3))) float*)a, x);
-}
 // the value of the same lane in the other half of the wave
 __device__ __forceinline__ float at_other_half(float x) { return __shfl_xor(x, 32, 64); }
 __device__ __forceinline__ f32x16 at_zero16()
@@ -193,10 +188,12 @@ template <int DP>
 __device__ __forceinline__ void at_load_rows(u32x4 (&f)[DP / 16], const mi_attn_rows& x, int64_t token, int head, int hd, int half)
 {
     const uint16_t* r = x.p + token * x.ts + (int64_t)head * x.hs;
+    const int most = (hd >> 3) - 1;
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) {
         const int c = 2 * s + half;
-        f[s] = c * 8 < hd ? *reinterpret_cast<const u32x4*>(r + c * 8) : u32x4{0, 0, 0, 0};
+        const u32x4 v = *reinterpret_cast<const u32x4*>(r + (c < most ? c : most) * 8);
+        f[s] = c <= most ? v : u32x4{0, 0, 0, 0};
     }
 }
 // ... and a 32-row operand block of a tile: lane's row 32 st + col
@@ -228,12 +225,24 @@ __device__ __forceinline__ void at_store_row(const mi_attn_rows& x, int64_t toke
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int d = 32 * dt + 8 * g + 4 * half;
-            if (d < hd) {
+            if (hd == DP || d < hd) {
                 uint2 o;
                 o.x = at_pack2<F16>(acc[dt][4 * g + 0] * f, acc[dt][4 * g + 1] * f);
                 o.y = at_pack2<F16>(acc[dt][4 * g + 2] * f, acc[dt][4 * g + 3] * f);
                 *reinterpret_cast<uint2*>(r + d) = o;
             }
+        }
+}
+// ... and as fp32, row `row` of a [rows][head_dim] array
+template <int DP>
+__device__ __forceinline__ void at_store_part(float* x, int64_t row, int hd, int half, const f32x16 (&acc)[DP / 32], float f)
+{
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int d = 32 * dt + 8 * g + 4 * half;
+            if (d < hd) *reinterpret_cast<float4*>(x + row * hd + d) = make_float4(acc[dt][4 * g] * f, acc[dt][4 * g + 1] * f, acc[dt][4 * g + 2] * f, acc[dt][4 * g + 3] * f);
         }
 }
 __device__ __forceinline__ void at_zero_rows(const mi_attn_rows& x, int64_t token0, int rows, int head, int hd)
@@ -261,13 +270,33 @@ __host__ __device__ __forceinline__ int at_bucket(const mi_attn_args& p, int r)
     }
     return b + (p.two_sided && r > 0 ? p.side : 0);
 }
+__device__ __forceinline__ float at_bias(const mi_attn_args& p, int head, int r)
+{
+    const float x = p.table[(int64_t)at_bucket(p, r) * p.heads + head];
+    return (fabsf(x) <= FLT_MAX ? fminf(fmaxf(x, -AT_BIAS_MOST), AT_BIAS_MOST) : x) * AT_LOG2E;
+}
 __device__ __forceinline__ void at_fill_bias(const mi_attn_args& p, int head, float* vec)
 {
     const int R = p.reach + AT_PAD;
-    for (int i = threadIdx.x; i < 2 * R + 1; i += blockDim.x) {
-        const float x = p.table[(int64_t)at_bucket(p, i - R) * p.heads + head];
-        vec[i] = (fabsf(x) <= FLT_MAX ? fminf(fmaxf(x, -AT_BIAS_MOST), AT_BIAS_MOST) : x) * AT_LOG2E;
+    for (int i = threadIdx.x; i < 2 * R + 1; i += blockDim.x) vec[i] = at_bias(p, head, i - R);
+}
+
+// Which of the 64 keys at k0 are keys of the sequence that the mask leaves (bit = key - k0); the wave's lanes ask for one each.
+__device__ __forceinline__ uint64_t at_keys(const int32_t* mask, int k0, int len, int lane)
+{
+    if (!mask && k0 + AT_KT <= len) return ~0ull;
+    const int key = k0 + lane;
+    return __builtin_amdgcn_ballot_w64(key < len && (!mask || mask[key < len ? key : len - 1] != 0));
+}
+// ... and of the 32 of block st those that this lane's query attends, bit 8 g + i for its register 4 g + i; ahead = query - k0
+__device__ __forceinline__ uint32_t at_allowed(const mi_attn_args& p, uint64_t keys, int st, int ahead, int half)
+{
+    uint32_t ok = (uint32_t)(keys >> (32 * st));
+    if (p.causal) {
+        const int lim = ahead - 32 * st;                               // the last attended key of the block
+        ok = lim >= 31 ? ok : lim < 0 ? 0u : ok & ((2u << lim) - 1u);
     }
+    return ok >> (4 * half);
 }
 
 // ---------------------------------------------------------------- forward
@@ -331,11 +360,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const mi_attn_args p)
         if (qw >= len || (p.causal && k0 > qw + 32 * QB - 1)) continue;  // nothing for this wave (it has met the barrier)
         const char* const Kt = lds + buf * 2 * TB;
         const char* const Vt = Kt + TB;
-        uint64_t keys = ~0ull;
-        if (mask || k0 + AT_KT > len) {
-            const int key = k0 + lane;
-            keys = __builtin_amdgcn_ballot_w64(key < len && (!mask || mask[key < len ? key : len - 1] != 0));
-        }
+        const uint64_t keys = at_keys(mask, k0, len, lane);
         const bool masked = ~keys != 0 || (p.causal && k0 + AT_KT - 1 > qw);
 
         f32x16 S[QB][2];
@@ -377,12 +402,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const mi_attn_args p)
             if (masked) {
 #pragma unroll
                 for (int st = 0; st < 2; ++st) {
-                    uint32_t ok = (uint32_t)(keys >> (32 * st));
-                    if (p.causal) {
-                        const int lim = q - k0 - 32 * st;              // the last attended key of this block
-                        ok = lim >= 31 ? ok : lim < 0 ? 0u : ok & ((2u << lim) - 1u);
-                    }
-                    ok >>= 4 * half;
+                    const uint32_t ok = at_allowed(p, keys, st, q - k0, half);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) S[b][st][i] = (ok >> (8 * (i >> 2) + (i & 3))) & 1u ? S[b][st][i] : -INFINITY;
                 }
@@ -450,22 +470,100 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const mi_attn_args p)
 // thousands of keys has p near fp16's subnormals), and ds = p (dp - D) takes the scale back out.
 template <bool F16> struct AtPScale { static constexpr float log2 = F16 ? 12.0f : 0.0f, up = F16 ? 4096.0f : 1.0f, down = F16 ? 1.0f / 4096.0f : 1.0f; };
 
+// D = sum_j p dp of every row.  rowsum(dout * out) is the same sum, but takes over the rounding of p and out in the forward pass,
+// which shows in rows of few keys (20 causal rows: dq and dk 1.65 x the plain rounding of their values, 1.4 with D exact).  So
+// where a block's keys fit the two tile buffers the sum is made from the scores, in fp32; longer rows take the dot product.
+template <int DP, bool F16, bool BIAS>
+__global__ __launch_bounds__(256, 2) void attn_delta_kernel(const mi_attn_args p)
+{
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    constexpr int BM = 128, TB = AtTile<DP>::BYTES;
+    float* const vec = reinterpret_cast<float*>(lds + 4 * TB);
+    int head, t, start, len, tile;
+    bool tail;
+    if (!at_work(p, head, t) || !at_find<BM>(p, t, start, len, tile, tail) || tail || tile * BM >= len) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, half = lane >> 5;
+    const int qw = tile * BM + wave * 32, q = qw + col;
+    const int kend = p.causal ? (tile * BM + BM < len ? tile * BM + BM : len) : len;
+    const int64_t tok = start + (q < len ? q : len - 1);
+    u32x4 df[DP / 16], qf[DP / 16];                                    // qf: rows of out, or of q
+    at_load_rows<DP>(df, p.dout, tok, head, p.hd, half);
+    float a = 0.0f, c = 0.0f;
+    if (kend > 2 * AT_KT) {
+        at_load_rows<DP>(qf, p.out, tok, head, p.hd, half);
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                a = __builtin_fmaf(at_lo<F16>(df[s][j]), at_lo<F16>(qf[s][j]), a);
+                a = __builtin_fmaf(at_hi<F16>(df[s][j]), at_hi<F16>(qf[s][j]), a);
+            }
+        c = half == 0 ? 1.0f : 0.0f;
+    } else {
+        at_load_rows<DP>(qf, p.q, tok, head, p.hd, half);
+        AtStage<DP, 4> ks, vs;
+        ks.init(p.k, start, len, head / p.group, p.hd, wave, lane);
+        vs.init(p.v, start, len, head / p.group, p.hd, wave, lane);
+        const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds;
+        const int32_t* const mask = p.key_mask ? p.key_mask + start : nullptr;
+        for (int k0 = 0; k0 < kend; k0 += AT_KT) {
+            ks.issue(k0, lds0 + k0 / AT_KT * 2 * TB, wave, mask);
+            vs.issue(k0, lds0 + k0 / AT_KT * 2 * TB + TB, wave, mask);
+        }
+        if constexpr (BIAS) at_fill_bias(p, head, vec);
+        float nl = p.lse[(int64_t)head * p.tokens + tok] * AT_LOG2E;
+        if (nl == -INFINITY) nl = INFINITY;                            // a row that attends nothing: p = 0
+        at_sync();
+        const int most = 2 * (p.reach + AT_PAD);
+        for (int k0 = 0; k0 < kend && qw < len; k0 += 32) {
+            if (p.causal && k0 > qw + 31) break;
+            const int st = (k0 >> 5) & 1, kt = k0 & ~(AT_KT - 1);
+            const char* const Kt = lds + kt / AT_KT * 2 * TB;
+            f32x16 S = at_zero16(), dP = at_zero16();
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s) S = at_mfma<F16>(at_rows<DP>(Kt, st, s, col, half), qf[s], S);
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s) dP = at_mfma<F16>(at_rows<DP>(Kt + TB, st, s, col, half), df[s], dP);
+            const uint32_t ok = at_allowed(p, at_keys(mask, kt, len, lane), st, q - kt, half);
+            const int at = k0 + 4 * half - q + p.reach + AT_PAD;       // may leave the vector where all of |r| is beyond reach
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float b = -nl;
+                if constexpr (BIAS) {
+                    int e = at + 8 * (i >> 2) + (i & 3);
+                    e = e < 0 ? 0 : e > most ? most : e;
+                    b += vec[e];
+                }
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], p.scale_log2, b));
+                const bool on = (ok >> (8 * (i >> 2) + (i & 3))) & 1u;
+                a += on ? x * dP[i] : 0.0f;
+                c += on ? x : 0.0f;
+            }
+        }
+    }
+    a += at_other_half(a);
+    c += at_other_half(c);
+    if (half == 0 && q < len) p.delta[(int64_t)head * p.tokens + tok] = c == 0.0f ? a : a / c;
+}
+
 // dQ: one block per (head, 32 NW query rows), like the forward pass: S^T = K Q^T and dP^T = V dO^T with the query on the lane,
-// dQ^T += K^T dS^T.  Writes D = rowsum(dout * out) for attn_dkv_kernel.
+// dQ^T += K^T dS^T.
 //
-// BIAS: the table's gradient.  D comes from the rounded `out`, good for ds as a 16-bit operand but not for sums over thousands of
-// keys, so the lane keeps, per bucket, A = sum p dp and C = sum p of its query (LDS, one column per lane, so the order of the
-// additions is fixed; a tile that lies in one bucket adds in registers), and at the end
+// BIAS: the table's gradient.  D from rounded rows is not good enough for sums over thousands of keys, so the lane keeps, per bucket, A = sum p dp and C = sum p of its query, and at the end
 //   dT[b] += (A_b - D C_b) / C  with  D = sum_b A_b / C, C = sum_b C_b  (= 1 but for the rounding of the saved lse).
+// A lane meets its keys in rising order and the buckets along them are runs, so the sums of the present bucket stay in registers
+// and are stored to the lane's own column in LDS as they grow: the last store of a run is the bucket's sum, nothing is read
+// back and no order is left open.  (Adding into LDS instead, ds_add_f32, cost 122 cycles an instruction: 427 us where this is
+// @DQ_RUNS@ us, 96 sequences up to 256, 12 heads of 32.)
 template <int DP, bool F16, bool BIAS, int NW>
 __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void attn_dq_kernel(const mi_attn_args p)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     constexpr int BM = 32 * NW, TB = AtTile<DP>::BYTES;
     const int R = p.reach + AT_PAD, nvec = 2 * R + 1;
-    float* const acc0 = reinterpret_cast<float*>(lds + 4 * TB);        // BIAS: [NW][A | C][buckets][64], then the two vectors
-    float* const vec = acc0 + NW * 2 * p.buckets * 64;
-    int* const bvec = reinterpret_cast<int*>(vec + nvec);              // element offset of the bucket's row in an accumulator
+    float2* const acc0 = reinterpret_cast<float2*>(lds + 4 * TB);      // BIAS: (A, C) [NW][buckets][64], then over r = -R .. R
+    float2* const vec = acc0 + NW * p.buckets * 64;                    // (bias, the bucket's row in acc0 as a whole number)
     int head, t, start, len, tile;
     bool tail;
     if (!at_work(p, head, t)) return;
@@ -487,37 +585,32 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void attn_dq_kernel(const
     vs.init(p.v, start, len, kvh, p.hd, wave, lane);
     const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds;
     const int32_t* const mask = p.key_mask ? p.key_mask + start : nullptr;
-    ks.issue(0, lds0, wave, mask);
-    vs.issue(0, lds0 + TB, wave, mask);
+    auto issue = [&](int k0, int buf) __attribute__((always_inline)) {
+        ks.issue(k0, lds0 + buf * 2 * TB, wave, mask);
+        vs.issue(k0, lds0 + buf * 2 * TB + TB, wave, mask);
+    };
+    issue(0, 0);
 
     u32x4 qf[DP / 16], df[DP / 16];
-    float D = 0.0f;
-    {
-        const int64_t tok = start + (q < len ? q : len - 1);
-        at_load_rows<DP>(qf, p.q, tok, head, p.hd, half);
-        at_load_rows<DP>(df, p.dout, tok, head, p.hd, half);
-        u32x4 of[DP / 16];
-        at_load_rows<DP>(of, p.out, tok, head, p.hd, half);
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                D = __builtin_fmaf(at_lo<F16>(df[s][j]), at_lo<F16>(of[s][j]), D);
-                D = __builtin_fmaf(at_hi<F16>(df[s][j]), at_hi<F16>(of[s][j]), D);
-            }
-        D += at_other_half(D);
-        if (half == 0 && q < len) p.delta[(int64_t)head * p.tokens + tok] = D;
-    }
-    float nl = p.lse[(int64_t)head * p.tokens + start + (q < len ? q : len - 1)] * AT_LOG2E;
+    const int64_t tok = start + (q < len ? q : len - 1);
+    at_load_rows<DP>(qf, p.q, tok, head, p.hd, half);
+    at_load_rows<DP>(df, p.dout, tok, head, p.hd, half);
+    const float D = p.delta[(int64_t)head * p.tokens + tok];
+    float nl = p.lse[(int64_t)head * p.tokens + tok] * AT_LOG2E;
     if (nl == -INFINITY) nl = INFINITY;                                // a row that attends nothing: p = 0
 
-    float* const accA = acc0 + wave * 2 * p.buckets * 64 + lane;
-    float* const accC = accA + p.buckets * 64;
-    float farA[2] = {0.0f, 0.0f}, farC[2] = {0.0f, 0.0f};
+    float2* const acc = acc0 + wave * p.buckets * 64 + lane;
+    float runA = 0.0f, runC = 0.0f;
+    int run = -1;                                                      // the present bucket's row
+    auto add = [&](int b, float a, float c) __attribute__((always_inline)) {
+        runA = (b == run ? runA : 0.0f) + a;
+        runC = (b == run ? runC : 0.0f) + c;
+        run = b;
+        acc[b] = make_float2(runA, runC);
+    };
     if constexpr (BIAS) {
-        at_fill_bias(p, head, vec);
-        for (int i = threadIdx.x; i < nvec; i += 64 * NW) bvec[i] = at_bucket(p, i - R) * 64;
-        for (int b = 0; b < 2 * p.buckets; ++b) accA[b * 64] = 0.0f;
+        for (int i = threadIdx.x; i < nvec; i += 64 * NW) vec[i] = make_float2(at_bias(p, head, i - R), __builtin_bit_cast(float, at_bucket(p, i - R) * 64));
+        for (int b = 0; b < p.buckets; ++b) acc[b * 64] = make_float2(0.0f, 0.0f);
     }
     f32x16 dQ[DP / 32];
 #pragma unroll
@@ -525,42 +618,29 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void attn_dq_kernel(const
 
     for (int k0 = 0, buf = 0; k0 < kend; k0 += AT_KT, buf ^= 1) {
         at_sync();
-        if (k0 + AT_KT < kend) {
-            ks.issue(k0 + AT_KT, lds0 + (buf ^ 1) * 2 * TB, wave, mask);
-            vs.issue(k0 + AT_KT, lds0 + (buf ^ 1) * 2 * TB + TB, wave, mask);
-        }
+        if (k0 + AT_KT < kend) issue(k0 + AT_KT, buf ^ 1);
         if (qw >= len || (p.causal && k0 > qw + 31)) continue;
         const char* const Kt = lds + buf * 2 * TB;
-        const char* const Vt = Kt + TB;
-        uint64_t keys = ~0ull;
-        if (mask || k0 + AT_KT > len) {
-            const int key = k0 + lane;
-            keys = __builtin_amdgcn_ballot_w64(key < len && (!mask || mask[key < len ? key : len - 1] != 0));
-        }
+        const uint64_t keys = at_keys(mask, k0, len, lane);
         const bool masked = ~keys != 0 || (p.causal && k0 + AT_KT - 1 > qw);
         const int rlo = k0 - (qw + 31), rhi = k0 + AT_KT - 1 - qw;
         const bool near = BIAS && rhi > -p.reach && rlo < p.reach;
-        const float shift = BIAS && !near ? vec[rhi <= -p.reach ? 0 : 2 * R] - nl : -nl;
-        const int at = k0 + 4 * half - q + R;
+        const float2 far = BIAS && !near ? vec[rhi <= -p.reach ? 0 : 2 * R] : make_float2(0.0f, 0.0f);
+        const float2* const bv = vec + (k0 + 4 * half - q + R);
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
             f32x16 S = at_zero16(), dP = at_zero16();
 #pragma unroll
             for (int s = 0; s < DP / 16; ++s) S = at_mfma<F16>(at_rows<DP>(Kt, st, s, col, half), qf[s], S);
 #pragma unroll
-            for (int s = 0; s < DP / 16; ++s) dP = at_mfma<F16>(at_rows<DP>(Vt, st, s, col, half), df[s], dP);
+            for (int s = 0; s < DP / 16; ++s) dP = at_mfma<F16>(at_rows<DP>(Kt + TB, st, s, col, half), df[s], dP);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float b = near ? vec[at + 32 * st + 8 * (i >> 2) + (i & 3)] : 0.0f;
-                S[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], p.scale_log2, b + shift));
+                const float b = near ? bv[32 * st + 8 * (i >> 2) + (i & 3)].x : far.x;
+                S[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], p.scale_log2, b - nl));
             }
             if (masked) {
-                uint32_t ok = (uint32_t)(keys >> (32 * st));
-                if (p.causal) {
-                    const int lim = q - k0 - 32 * st;
-                    ok = lim >= 31 ? ok : lim < 0 ? 0u : ok & ((2u << lim) - 1u);
-                }
-                ok >>= 4 * half;
+                const uint32_t ok = at_allowed(p, keys, st, q - k0, half);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const bool on = (ok >> (8 * (i >> 2) + (i & 3))) & 1u;
@@ -571,18 +651,13 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void attn_dq_kernel(const
             if constexpr (BIAS) {
                 if (near) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int b = bvec[at + 32 * st + 8 * (i >> 2) + (i & 3)];
-                        at_lds_add(accA + b, S[i] * dP[i]);
-                        at_lds_add(accC + b, S[i]);
-                    }
+                    for (int i = 0; i < 16; ++i)
+                        add(__builtin_bit_cast(int, bv[32 * st + 8 * (i >> 2) + (i & 3)].y), S[i] * dP[i], S[i]);
                 } else {
                     float a = 0.0f, c = 0.0f;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) { a = __builtin_fmaf(S[i], dP[i], a); c += S[i]; }
-                    const int side = rhi <= -p.reach ? 0 : 1;
-                    farA[0] += side == 0 ? a : 0.0f; farC[0] += side == 0 ? c : 0.0f;
-                    farA[1] += side == 1 ? a : 0.0f; farC[1] += side == 1 ? c : 0.0f;
+                    add(__builtin_bit_cast(int, far.y), a, c);
                 }
             }
 #pragma unroll
@@ -598,36 +673,33 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void attn_dq_kernel(const
     }
     if (q < len) at_store_row<DP, F16>(p.dq, start + q, head, p.hd, half, dQ, p.scale);
     if constexpr (BIAS) {
-        at_lds_add(accA + bvec[0], farA[0]);
-        at_lds_add(accC + bvec[0], farC[0]);
-        at_lds_add(accA + bvec[nvec - 1], farA[1]);
-        at_lds_add(accC + bvec[nvec - 1], farC[1]);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         float a = 0.0f, c = 0.0f;
-        for (int b = 0; b < p.buckets; ++b) { a += accA[b * 64]; c += accC[b * 64]; }
+        for (int b = 0; b < p.buckets; ++b) { a += acc[b * 64].x; c += acc[b * 64].y; }
         a += at_other_half(a);
         c += at_other_half(c);
         const bool on = q < len && c > 0.0f;
         const float w = on ? 1.0f / c : 0.0f, Dx = on ? a / c : 0.0f;
-        for (int b = 0; b < p.buckets; ++b) accA[b * 64] = on ? (accA[b * 64] - Dx * accC[b * 64]) * w : 0.0f;
+        for (int b = 0; b < p.buckets; ++b) acc[b * 64].x = on ? (acc[b * 64].x - Dx * acc[b * 64].y) * w : 0.0f;
         at_sync();
         // bucket b of the block: lane b of wave w sums its wave's row b (from a different column on each lane), then the waves
         float sum = 0.0f;
         if (lane < p.buckets)
-            for (int i = 0; i < 64; ++i) sum += acc0[wave * 2 * p.buckets * 64 + lane * 64 + ((i + lane) & 63)];
-        at_sync();
-        vec[wave * 64 + lane] = sum;                                   // (over the two vectors, 390 words and more, which have been read)
+            for (int i = 0; i < 64; ++i) sum += acc0[(wave * p.buckets + lane) * 64 + ((i + lane) & 63)].x;
+        float* const sums = reinterpret_cast<float*>(vec);             // (the vector, 390 words and more, has been read)
+        sums[wave * 64 + lane] = sum;
         at_sync();
         if (wave == 0) {
-            float all = vec[lane];
-            for (int w2 = 1; w2 < NW; ++w2) all += vec[w2 * 64 + lane];
+            float all = sums[lane];
+            for (int w2 = 1; w2 < NW; ++w2) all += sums[w2 * 64 + lane];
             part[lane] = all;
         }
     }
 }
 
-// dK, dV: one block per (key head, 128 keys), a wave per 32 keys, over the tiles of 64 query rows of every query head of the
-// group: S = Q K^T and dP = dO V^T with the key on the lane, dV^T += dO^T P, dK^T += Q^T dS.  The group's sum stays in fp32.
+// dK, dV: one block per (key head, share of its query heads, 128 keys), a wave per 32 keys, over the tiles of 64 query rows of
+// the share's heads: S = Q K^T and dP = dO V^T with the key on the lane, dV^T += dO^T P, dK^T += Q^T dS.  Where one block per key
+// head and tile would leave CUs idle the group's heads are shared out over `splits` blocks, whose fp32 sums attn_join_kernel
+// adds in the heads' order.
 template <int DP, bool F16, bool BIAS>
 __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(const mi_attn_args p)
 {
@@ -638,7 +710,11 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(const 
     int kvh, t, start, len, tile;
     bool tail;
     if (!at_work(p, kvh, t) || !at_find<BM>(p, t, start, len, tile, tail)) return;
+    const int share = kvh % p.splits, heads = p.group / p.splits;      // (units are key heads x shares)
+    kvh /= p.splits;
+    const int head0 = kvh * p.group + share * heads;
     if (tail) {
+        if (share != 0) return;
         const int n = len - tile * BM < BM ? len - tile * BM : BM;
         at_zero_rows(p.dk, start + tile * BM, n, kvh, p.hd);
         at_zero_rows(p.dv, start + tile * BM, n, kvh, p.hd);
@@ -656,11 +732,11 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(const 
 
     const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds;
     const int qfirst = p.causal ? tile * BM / AT_KT * AT_KT : 0;       // earlier queries attend no key of this block
-    const int nq = (len - qfirst + AT_KT - 1) / AT_KT, n = nq * p.group;
+    const int nq = (len - qfirst + AT_KT - 1) / AT_KT, n = nq * heads;
     AtStage<DP, 4> qs, ds;
     float rowreg = 0.0f;
     auto issue = [&](int it, int buf) __attribute__((always_inline)) {
-        const int head = kvh * p.group + it / nq, q0 = qfirst + it % nq * AT_KT;
+        const int head = head0 + it / nq, q0 = qfirst + it % nq * AT_KT;
         qs.init(p.q, start, len, head, p.hd, wave, lane);
         ds.init(p.dout, start, len, head, p.hd, wave, lane);
         qs.issue(q0, lds0 + buf * 2 * TB, wave);
@@ -684,7 +760,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(const 
     int bias_head = -1;
     for (int it = 0, buf = 0; it < n; ++it, buf ^= 1) {
         if (wave < 2) rowv[buf * 128 + wave * 64 + lane] = rowreg;
-        const int head = kvh * p.group + it / nq, q0 = qfirst + it % nq * AT_KT;
+        const int head = head0 + it / nq, q0 = qfirst + it % nq * AT_KT;
         if constexpr (BIAS) {
             if (head != bias_head) {
                 if (bias_head >= 0) at_sync();                         // the last head's vector has been read
@@ -751,9 +827,37 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(const 
 #pragma unroll
             for (int dt = 0; dt < DP / 32; ++dt) { dK[dt] = at_zero16(); dV[dt] = at_zero16(); }
         }
-        at_store_row<DP, F16>(p.dk, start + key, kvh, p.hd, half, dK, p.scale);
-        at_store_row<DP, F16>(p.dv, start + key, kvh, p.hd, half, dV, AtPScale<F16>::down);
+        if (p.splits == 1) {
+            at_store_row<DP, F16>(p.dk, start + key, kvh, p.hd, half, dK, p.scale);
+            at_store_row<DP, F16>(p.dv, start + key, kvh, p.hd, half, dV, AtPScale<F16>::down);
+        } else {
+            at_store_part<DP>(p.parts_kv, ((int64_t)(2 * share) * p.tokens + start + key) * (p.heads / p.group) + kvh, p.hd, half, dK, p.scale);
+            at_store_part<DP>(p.parts_kv, ((int64_t)(2 * share + 1) * p.tokens + start + key) * (p.heads / p.group) + kvh, p.hd, half, dV, AtPScale<F16>::down);
+        }
     }
+}
+
+// dk and dv from the shares' sums ([share][dk | dv][token][key head][head_dim] fp32), 8 elements a thread
+template <bool F16>
+__global__ __launch_bounds__(256) void attn_join_kernel(const mi_attn_args p)
+{
+    const int per = p.hd >> 3, kvh = p.heads / p.group;
+    const int64_t n = p.tokens * kvh * per, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const int64_t row = i / per, token = row / kvh;
+    if (p.offsets && (token < p.offsets[0] || token >= p.offsets[p.nseq])) return;   // no sequence's: left, or zeroed by the tail's block
+    const mi_attn_rows& x = blockIdx.y ? p.dv : p.dk;
+    float sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int s = 0; s < p.splits; ++s) {
+        const float4* src = reinterpret_cast<const float4*>(p.parts_kv + (((int64_t)(2 * s + blockIdx.y) * p.tokens) * kvh + row) * p.hd + (i % per) * 8);
+        const float4 a = src[0], b = src[1];
+        sum[0] += a.x; sum[1] += a.y; sum[2] += a.z; sum[3] += a.w;
+        sum[4] += b.x; sum[5] += b.y; sum[6] += b.z; sum[7] += b.w;
+    }
+    u32x4 o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = at_pack2<F16>(sum[2 * j], sum[2 * j + 1]);
+    *reinterpret_cast<u32x4*>(x.p + token * x.ts + (row % kvh) * x.hs + (i % per) * 8) = o;
 }
 
 // dT[b][head] = the sum of the blocks' partial sums, in the tiles' order within each of 16 strides
@@ -818,12 +922,26 @@ int mi_launch_attention(hipStream_t st, mi_attn_args a, int dtype)
 static int at_dq_waves(const mi_attn_args& a) { return a.table && a.buckets > 32 ? 2 : 4; }
 static int64_t at_dq_tiles(int64_t tokens, int64_t nseq, int BM) { return tokens / BM + nseq + 1; }
 
+// Shares of a group's query heads in the dK / dV kernel: the fewest that give AT_DKV_BLOCKS blocks (two per CU, four rounds, so
+// that a causal sequence's long first tiles even out), all heads at most.  1 x 8,191 causal, 8 heads on 2 key heads of 128:
+// 128 blocks 1,620 us, 512 blocks @DKV_SPLIT@ us.
+#define AT_DKV_BLOCKS 2048
+static int at_dkv_splits(const mi_attn_args& a)
+{
+    const int64_t blocks = (int64_t)(a.heads / a.group) * (a.tokens / 128 + a.nseq);
+    for (int s = 1; s < a.group; ++s)
+        if (a.group % s == 0 && blocks * s >= AT_DKV_BLOCKS) return s;
+    return a.group;
+}
+
 size_t mi_attn_backward_bytes(const mi_attn_args& a)
 {
     const size_t delta = mi_round_up((int64_t)a.heads * a.tokens * 4, 256);
+    const int splits = at_dkv_splits(a);
+    const size_t join = splits > 1 ? (size_t)mi_round_up((int64_t)splits * 2 * a.tokens * (a.heads / a.group) * a.hd * 4, 256) : 0;
     const int64_t tiles = a.offsets ? at_dq_tiles(a.tokens, a.nseq, 32 * at_dq_waves(a))
                                     : (int64_t)a.nseq * ((a.uniform_len + 32 * at_dq_waves(a) - 1) / (32 * at_dq_waves(a)));
-    return delta + (a.table ? (size_t)(a.heads * tiles) * MI_ATTN_MAX_BUCKETS * 4 : 0);
+    return delta + join + (a.table ? (size_t)(a.heads * tiles) * MI_ATTN_MAX_BUCKETS * 4 : 0);
 }
 
 template <int DP, bool F16, bool BIAS, int NW>
@@ -839,9 +957,23 @@ static int launch_dq(hipStream_t st, mi_attn_args& a)
     return MI_OK;
 }
 
+template <int DP, bool F16, bool BIAS>
+static int launch_delta(hipStream_t st, mi_attn_args& a)
+{
+    const unsigned grid = at_schedule(&a, a.heads, 128);
+    if (grid == 0) return MI_OK;
+    const size_t smem = 4 * AtTile<DP>::BYTES + (BIAS ? (size_t)(2 * (a.reach + AT_PAD) + 1) * 4 : 0);
+    MI_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(attn_delta_kernel<DP, F16, BIAS>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    attn_delta_kernel<DP, F16, BIAS><<<grid, 256, smem, st>>>(a);
+    MI_HIP(hipGetLastError());
+    return MI_OK;
+}
+
 template <int DP, bool F16>
 static int launch_bwd(hipStream_t st, mi_attn_args& a)
 {
+    if (a.table) MI_TRY((launch_delta<DP, F16, true>(st, a)));
+    else MI_TRY((launch_delta<DP, F16, false>(st, a)));
     if (!a.table) MI_TRY((launch_dq<DP, F16, false, 4>(st, a)));
     else if (at_dq_waves(a) == 4) MI_TRY((launch_dq<DP, F16, true, 4>(st, a)));
     else MI_TRY((launch_dq<DP, F16, true, 2>(st, a)));
@@ -849,7 +981,7 @@ static int launch_bwd(hipStream_t st, mi_attn_args& a)
         attn_dtable_kernel<<<(unsigned)a.heads, 1024, 0, st>>>(a);
         MI_HIP(hipGetLastError());
     }
-    const unsigned grid = at_schedule(&a, a.heads / a.group, 128);
+    const unsigned grid = at_schedule(&a, a.heads / a.group * a.splits, 128);
     if (grid == 0) return MI_OK;
     const size_t smem = 4 * AtTile<DP>::BYTES + 1024 + (a.table ? (size_t)(2 * (a.reach + AT_PAD) + 1) * 4 : 0);
     if (a.table) {
@@ -860,13 +992,19 @@ static int launch_bwd(hipStream_t st, mi_attn_args& a)
         attn_dkv_kernel<DP, F16, false><<<grid, 256, smem, st>>>(a);
     }
     MI_HIP(hipGetLastError());
+    if (a.splits > 1) {
+        attn_join_kernel<F16><<<dim3((unsigned)((a.tokens * (a.heads / a.group) * (a.hd >> 3) + 255) / 256), 2), 256, 0, st>>>(a);
+        MI_HIP(hipGetLastError());
+    }
     return MI_OK;
 }
 
 int mi_launch_attention_backward(hipStream_t st, mi_attn_args a, int dtype, void* workspace)
 {
     a.delta = (float*)workspace;
-    a.partial = (float*)((char*)workspace + mi_round_up((int64_t)a.heads * a.tokens * 4, 256));
+    a.splits = at_dkv_splits(a);
+    a.parts_kv = (float*)((char*)workspace + mi_round_up((int64_t)a.heads * a.tokens * 4, 256));
+    a.partial = (float*)((char*)a.parts_kv + (a.splits > 1 ? mi_round_up((int64_t)a.splits * 2 * a.tokens * (a.heads / a.group) * a.hd * 4, 256) : 0));
     const bool f16 = dtype == MI_DTYPE_F16;
     if (a.hd <= 32) return f16 ? launch_bwd<32, true>(st, a) : launch_bwd<32, false>(st, a);
     if (a.hd <= 64) return f16 ? launch_bwd<64, true>(st, a) : launch_bwd<64, false>(st, a);
@@ -971,7 +1109,7 @@ extern "C" int mi_attention_dev(mi_ctx* ctx, const mi_attention_config* cfg, int
 extern "C" int mi_attention_backward_workspace(const mi_attention_config* cfg, int64_t tokens, int64_t nseq, int packed, size_t* bytes)
 {
     MI_REQUIRE(cfg && bytes, "mi_attention_backward_workspace: NULL argument");
-    MI_REQUIRE(cfg->heads > 0 && tokens >= 0 && nseq >= 0 && (packed || nseq == 0 || tokens % nseq == 0), "mi_attention_backward_workspace: bad argument");
+    MI_REQUIRE(cfg->heads > 0 && cfg->kv_heads > 0 && cfg->heads % cfg->kv_heads == 0 && cfg->head_dim > 0 && tokens >= 0 && nseq >= 0 && (packed || nseq == 0 || tokens % nseq == 0), "mi_attention_backward_workspace: bad argument");
     mi_attn_args a;
     static const int32_t some = 0;
     static const float one = 0.0f;
@@ -981,6 +1119,8 @@ extern "C" int mi_attention_backward_workspace(const mi_attention_config* cfg, i
     }
     a.offsets = packed ? &some : nullptr;
     a.heads = cfg->heads;
+    a.group = cfg->heads / cfg->kv_heads;
+    a.hd = cfg->head_dim;
     a.tokens = tokens;
     a.nseq = (int)nseq;
     a.uniform_len = packed || nseq == 0 ? 0 : (int)(tokens / nseq);
