@@ -471,8 +471,9 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const mi_attn_args p)
 template <bool F16> struct AtPScale { static constexpr float log2 = F16 ? 12.0f : 0.0f, up = F16 ? 4096.0f : 1.0f, down = F16 ? 1.0f / 4096.0f : 1.0f; };
 
 // D = sum_j p dp of every row.  rowsum(dout * out) is the same sum, but takes over the rounding of p and out in the forward pass,
-// which shows in rows of few keys (20 causal rows: dq and dk 1.65 x the plain rounding of their values, 1.4 with D exact).  So
-// where a block's keys fit the two tile buffers the sum is made from the scores, in fp32; longer rows take the dot product.
+// which shows in rows of few keys (20 causal rows: dq and dk 1.65 x the plain rounding of their values, 1.4 with D exact) and in
+// the table's gradient, a sum of many ds that nearly cancel.  So with a bias, for rows of up to 128 keys, and for up to 512 where
+// a mask may leave few of them, the sum is made from the scores, in fp32; other rows take the dot product.
 template <int DP, bool F16, bool BIAS>
 __global__ __launch_bounds__(256, 2) void attn_delta_kernel(const mi_attn_args p)
 {
@@ -484,13 +485,15 @@ __global__ __launch_bounds__(256, 2) void attn_delta_kernel(const mi_attn_args p
     if (!at_work(p, head, t) || !at_find<BM>(p, t, start, len, tile, tail) || tail || tile * BM >= len) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
+    if (p.causal) tile = (len + BM - 1) / BM - 1 - tile;
     const int qw = tile * BM + wave * 32, q = qw + col;
     const int kend = p.causal ? (tile * BM + BM < len ? tile * BM + BM : len) : len;
     const int64_t tok = start + (q < len ? q : len - 1);
+    const int32_t* const mask = p.key_mask ? p.key_mask + start : nullptr;
     u32x4 df[DP / 16], qf[DP / 16];                                    // qf: rows of out, or of q
     at_load_rows<DP>(df, p.dout, tok, head, p.hd, half);
     float a = 0.0f, c = 0.0f;
-    if (kend > 2 * AT_KT) {
+    if (!BIAS && kend > (mask ? 512 : 128)) {
         at_load_rows<DP>(qf, p.out, tok, head, p.hd, half);
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s)
@@ -506,39 +509,54 @@ __global__ __launch_bounds__(256, 2) void attn_delta_kernel(const mi_attn_args p
         ks.init(p.k, start, len, head / p.group, p.hd, wave, lane);
         vs.init(p.v, start, len, head / p.group, p.hd, wave, lane);
         const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds;
-        const int32_t* const mask = p.key_mask ? p.key_mask + start : nullptr;
-        for (int k0 = 0; k0 < kend; k0 += AT_KT) {
-            ks.issue(k0, lds0 + k0 / AT_KT * 2 * TB, wave, mask);
-            vs.issue(k0, lds0 + k0 / AT_KT * 2 * TB + TB, wave, mask);
-        }
+        ks.issue(0, lds0, wave, mask);
+        vs.issue(0, lds0 + TB, wave, mask);
         if constexpr (BIAS) at_fill_bias(p, head, vec);
         float nl = p.lse[(int64_t)head * p.tokens + tok] * AT_LOG2E;
         if (nl == -INFINITY) nl = INFINITY;                            // a row that attends nothing: p = 0
-        at_sync();
-        const int most = 2 * (p.reach + AT_PAD);
-        for (int k0 = 0; k0 < kend && qw < len; k0 += 32) {
-            if (p.causal && k0 > qw + 31) break;
-            const int st = (k0 >> 5) & 1, kt = k0 & ~(AT_KT - 1);
-            const char* const Kt = lds + kt / AT_KT * 2 * TB;
-            f32x16 S = at_zero16(), dP = at_zero16();
+        const int R = p.reach + AT_PAD;
+        for (int k0 = 0, buf = 0; k0 < kend; k0 += AT_KT, buf ^= 1) {
+            at_sync();
+            if (k0 + AT_KT < kend) {
+                ks.issue(k0 + AT_KT, lds0 + (buf ^ 1) * 2 * TB, wave, mask);
+                vs.issue(k0 + AT_KT, lds0 + (buf ^ 1) * 2 * TB + TB, wave, mask);
+            }
+            if (qw >= len || (p.causal && k0 > qw + 31)) continue;
+            const char* const Kt = lds + buf * 2 * TB;
+            const uint64_t keys = at_keys(mask, k0, len, lane);
+            const bool masked = ~keys != 0 || (p.causal && k0 + AT_KT - 1 > qw);
+            const int rlo = k0 - (qw + 31), rhi = k0 + AT_KT - 1 - qw;
+            const bool near = BIAS && rhi > -p.reach && rlo < p.reach;
+            const float far = BIAS && !near ? vec[rhi <= -p.reach ? 0 : 2 * R] - nl : -nl;
+            const float* const bv = vec + (k0 + 4 * half - q + R);
 #pragma unroll
-            for (int s = 0; s < DP / 16; ++s) S = at_mfma<F16>(at_rows<DP>(Kt, st, s, col, half), qf[s], S);
+            for (int st = 0; st < 2; ++st) {
+                f32x16 S = at_zero16(), dP = at_zero16();
 #pragma unroll
-            for (int s = 0; s < DP / 16; ++s) dP = at_mfma<F16>(at_rows<DP>(Kt + TB, st, s, col, half), df[s], dP);
-            const uint32_t ok = at_allowed(p, at_keys(mask, kt, len, lane), st, q - kt, half);
-            const int at = k0 + 4 * half - q + p.reach + AT_PAD;       // may leave the vector where all of |r| is beyond reach
+                for (int s = 0; s < DP / 16; ++s) S = at_mfma<F16>(at_rows<DP>(Kt, st, s, col, half), qf[s], S);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float b = -nl;
-                if constexpr (BIAS) {
-                    int e = at + 8 * (i >> 2) + (i & 3);
-                    e = e < 0 ? 0 : e > most ? most : e;
-                    b += vec[e];
+                for (int s = 0; s < DP / 16; ++s) dP = at_mfma<F16>(at_rows<DP>(Kt + TB, st, s, col, half), df[s], dP);
+                if (near) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) S[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], p.scale_log2, bv[32 * st + 8 * (i >> 2) + (i & 3)] - nl));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) S[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], p.scale_log2, far));
                 }
-                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], p.scale_log2, b));
-                const bool on = (ok >> (8 * (i >> 2) + (i & 3))) & 1u;
-                a += on ? x * dP[i] : 0.0f;
-                c += on ? x : 0.0f;
+                if (masked) {
+                    const uint32_t ok = at_allowed(p, keys, st, q - k0, half);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const bool on = (ok >> (8 * (i >> 2) + (i & 3))) & 1u;
+                        S[i] = on ? S[i] : 0.0f;
+                        dP[i] = on ? dP[i] : 0.0f;
+                    }
+                }
+                float a1 = 0.0f, c1 = 0.0f;                            // (short chains: a long row's sums stay exact to fp32's last bits)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) { a1 = __builtin_fmaf(S[i], dP[i], a1); c1 += S[i]; }
+                a += a1;
+                c += c1;
             }
         }
     }
@@ -547,23 +565,22 @@ __global__ __launch_bounds__(256, 2) void attn_delta_kernel(const mi_attn_args p
     if (half == 0 && q < len) p.delta[(int64_t)head * p.tokens + tok] = c == 0.0f ? a : a / c;
 }
 
-// dQ: one block per (head, 32 NW query rows), like the forward pass: S^T = K Q^T and dP^T = V dO^T with the query on the lane,
+// dQ: one block per (head, 128 query rows), like the forward pass: S^T = K Q^T and dP^T = V dO^T with the query on the lane,
 // dQ^T += K^T dS^T.
 //
-// BIAS: the table's gradient.  D from rounded rows is not good enough for sums over thousands of keys, so the lane keeps, per bucket, A = sum p dp and C = sum p of its query, and at the end
-//   dT[b] += (A_b - D C_b) / C  with  D = sum_b A_b / C, C = sum_b C_b  (= 1 but for the rounding of the saved lse).
-// A lane meets its keys in rising order and the buckets along them are runs, so the sums of the present bucket stay in registers
-// and are stored to the lane's own column in LDS as they grow: the last store of a run is the bucket's sum, nothing is read
-// back and no order is left open.  (Adding into LDS instead, ds_add_f32, cost 122 cycles an instruction: 427 us where this is
-// @DQ_RUNS@ us, 96 sequences up to 256, 12 heads of 32.)
-template <int DP, bool F16, bool BIAS, int NW>
-__global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void attn_dq_kernel(const mi_attn_args p)
+// BIAS: the table's gradient is the sum of ds along the diagonals r = key - query.  A 32 x 32 block of ds goes through a skewed
+// image in LDS, element (key, query) at [query][key - query + 31], so that lane l finds a diagonal in column l (the positions a row
+// never writes hold the zeros they started with); the 63 sums are added to the wave's vector over r.  A tile of one bucket adds
+// in registers.  Every sum has one owner and a fixed order.  @DQ_BIAS@
+template <int DP, bool F16, bool BIAS>
+__global__ __launch_bounds__(256, 2) void attn_dq_kernel(const mi_attn_args p)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    constexpr int BM = 32 * NW, TB = AtTile<DP>::BYTES;
+    constexpr int BM = 128, TB = AtTile<DP>::BYTES;
     const int R = p.reach + AT_PAD, nvec = 2 * R + 1;
-    float2* const acc0 = reinterpret_cast<float2*>(lds + 4 * TB);      // BIAS: (A, C) [NW][buckets][64], then over r = -R .. R
-    float2* const vec = acc0 + NW * p.buckets * 64;                    // (bias, the bucket's row in acc0 as a whole number)
+    float* const skew0 = reinterpret_cast<float*>(lds + 4 * TB);       // BIAS: [4][32][64], the waves' images
+    float* const vec = skew0 + 4 * 32 * 64;                            // the bias over r
+    float* const dvec0 = vec + nvec;                                   // [4][nvec], the waves' sums over r
     int head, t, start, len, tile;
     bool tail;
     if (!at_work(p, head, t)) return;
@@ -580,16 +597,13 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void attn_dq_kernel(const
     const int kend = p.causal ? (tile * BM + BM < len ? tile * BM + BM : len) : len;
     const int kvh = head / p.group;
 
-    AtStage<DP, NW> ks, vs;
+    AtStage<DP, 4> ks, vs;
     ks.init(p.k, start, len, kvh, p.hd, wave, lane);
     vs.init(p.v, start, len, kvh, p.hd, wave, lane);
     const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds;
     const int32_t* const mask = p.key_mask ? p.key_mask + start : nullptr;
-    auto issue = [&](int k0, int buf) __attribute__((always_inline)) {
-        ks.issue(k0, lds0 + buf * 2 * TB, wave, mask);
-        vs.issue(k0, lds0 + buf * 2 * TB + TB, wave, mask);
-    };
-    issue(0, 0);
+    ks.issue(0, lds0, wave, mask);
+    vs.issue(0, lds0 + TB, wave, mask);
 
     u32x4 qf[DP / 16], df[DP / 16];
     const int64_t tok = start + (q < len ? q : len - 1);
@@ -597,20 +611,16 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void attn_dq_kernel(const
     at_load_rows<DP>(df, p.dout, tok, head, p.hd, half);
     const float D = p.delta[(int64_t)head * p.tokens + tok];
     float nl = p.lse[(int64_t)head * p.tokens + tok] * AT_LOG2E;
-    if (nl == -INFINITY) nl = INFINITY;                                // a row that attends nothing: p = 0
+    if (nl == -INFINITY || q >= len) nl = INFINITY;                    // a row that attends nothing, or is none: p = 0
 
-    float2* const acc = acc0 + wave * p.buckets * 64 + lane;
-    float runA = 0.0f, runC = 0.0f;
-    int run = -1;                                                      // the present bucket's row
-    auto add = [&](int b, float a, float c) __attribute__((always_inline)) {
-        runA = (b == run ? runA : 0.0f) + a;
-        runC = (b == run ? runC : 0.0f) + c;
-        run = b;
-        acc[b] = make_float2(runA, runC);
-    };
+    float* const skew = skew0 + wave * 32 * 64;
+    float* const dvec = dvec0 + wave * nvec;
+    float farS[2] = {0.0f, 0.0f};                                      // sums of the tiles of one bucket, before and behind
     if constexpr (BIAS) {
-        for (int i = threadIdx.x; i < nvec; i += 64 * NW) vec[i] = make_float2(at_bias(p, head, i - R), __builtin_bit_cast(float, at_bucket(p, i - R) * 64));
-        for (int b = 0; b < p.buckets; ++b) acc[b * 64] = make_float2(0.0f, 0.0f);
+        at_fill_bias(p, head, vec);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) skew[i * 64 + lane] = 0.0f;
+        for (int i = lane; i < nvec; i += 64) dvec[i] = 0.0f;
     }
     f32x16 dQ[DP / 32];
 #pragma unroll
@@ -618,15 +628,18 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void attn_dq_kernel(const
 
     for (int k0 = 0, buf = 0; k0 < kend; k0 += AT_KT, buf ^= 1) {
         at_sync();
-        if (k0 + AT_KT < kend) issue(k0 + AT_KT, buf ^ 1);
+        if (k0 + AT_KT < kend) {
+            ks.issue(k0 + AT_KT, lds0 + (buf ^ 1) * 2 * TB, wave, mask);
+            vs.issue(k0 + AT_KT, lds0 + (buf ^ 1) * 2 * TB + TB, wave, mask);
+        }
         if (qw >= len || (p.causal && k0 > qw + 31)) continue;
         const char* const Kt = lds + buf * 2 * TB;
         const uint64_t keys = at_keys(mask, k0, len, lane);
         const bool masked = ~keys != 0 || (p.causal && k0 + AT_KT - 1 > qw);
         const int rlo = k0 - (qw + 31), rhi = k0 + AT_KT - 1 - qw;
         const bool near = BIAS && rhi > -p.reach && rlo < p.reach;
-        const float2 far = BIAS && !near ? vec[rhi <= -p.reach ? 0 : 2 * R] : make_float2(0.0f, 0.0f);
-        const float2* const bv = vec + (k0 + 4 * half - q + R);
+        const float far = BIAS && !near ? vec[rhi <= -p.reach ? 0 : 2 * R] - nl : -nl;
+        const float* const bv = vec + (k0 + 4 * half - q + R);
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
             f32x16 S = at_zero16(), dP = at_zero16();
@@ -634,38 +647,43 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void attn_dq_kernel(const
             for (int s = 0; s < DP / 16; ++s) S = at_mfma<F16>(at_rows<DP>(Kt, st, s, col, half), qf[s], S);
 #pragma unroll
             for (int s = 0; s < DP / 16; ++s) dP = at_mfma<F16>(at_rows<DP>(Kt + TB, st, s, col, half), df[s], dP);
+            if (near) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float b = near ? bv[32 * st + 8 * (i >> 2) + (i & 3)].x : far.x;
-                S[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], p.scale_log2, b - nl));
+                for (int i = 0; i < 16; ++i) S[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], p.scale_log2, bv[32 * st + 8 * (i >> 2) + (i & 3)] - nl));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) S[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], p.scale_log2, far));
             }
+            // ds, over dp
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dP[i] = S[i] * (dP[i] - D);
             if (masked) {
                 const uint32_t ok = at_allowed(p, keys, st, q - k0, half);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const bool on = (ok >> (8 * (i >> 2) + (i & 3))) & 1u;
-                    S[i] = on ? S[i] : 0.0f;
-                    dP[i] = on ? dP[i] : 0.0f;
-                }
+                for (int i = 0; i < 16; ++i) dP[i] = (ok >> (8 * (i >> 2) + (i & 3))) & 1u ? dP[i] : 0.0f;
             }
             if constexpr (BIAS) {
                 if (near) {
+                    float* const at = skew + col * 63 + 31 + 4 * half;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        add(__builtin_bit_cast(int, bv[32 * st + 8 * (i >> 2) + (i & 3)].y), S[i] * dP[i], S[i]);
+                    for (int i = 0; i < 16; ++i) at[8 * (i >> 2) + (i & 3)] = dP[i];
+                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sum[i & 3] += skew[i * 64 + lane];
+                    if (lane < 63) dvec[rlo + 32 * st + R + lane] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 } else {
-                    float a = 0.0f, c = 0.0f;
+                    float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) { a = __builtin_fmaf(S[i], dP[i], a); c += S[i]; }
-                    add(__builtin_bit_cast(int, far.y), a, c);
+                    for (int i = 0; i < 16; ++i) sum[i & 1] += dP[i];
+                    farS[0] += rhi <= -p.reach ? sum[0] + sum[1] : 0.0f;
+                    farS[1] += rhi <= -p.reach ? 0.0f : sum[0] + sum[1];
                 }
             }
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
                 u32x4 sf;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    sf[i] = at_pack2<F16>(S[8 * kk + 2 * i] * (dP[8 * kk + 2 * i] - D), S[8 * kk + 2 * i + 1] * (dP[8 * kk + 2 * i + 1] - D));
+                for (int i = 0; i < 4; ++i) sf[i] = at_pack2<F16>(dP[8 * kk + 2 * i], dP[8 * kk + 2 * i + 1]);
 #pragma unroll
                 for (int dt = 0; dt < DP / 32; ++dt) dQ[dt] = at_mfma<F16>(at_cols<DP>(Kt, 2 * st + kk, dt, lane), sf, dQ[dt]);
             }
@@ -673,26 +691,31 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void attn_dq_kernel(const
     }
     if (q < len) at_store_row<DP, F16>(p.dq, start + q, head, p.hd, half, dQ, p.scale);
     if constexpr (BIAS) {
-        float a = 0.0f, c = 0.0f;
-        for (int b = 0; b < p.buckets; ++b) { a += acc[b * 64].x; c += acc[b * 64].y; }
-        a += at_other_half(a);
-        c += at_other_half(c);
-        const bool on = q < len && c > 0.0f;
-        const float w = on ? 1.0f / c : 0.0f, Dx = on ? a / c : 0.0f;
-        for (int b = 0; b < p.buckets; ++b) acc[b * 64].x = on ? (acc[b * 64].x - Dx * acc[b * 64].y) * w : 0.0f;
-        at_sync();
-        // bucket b of the block: lane b of wave w sums its wave's row b (from a different column on each lane), then the waves
-        float sum = 0.0f;
-        if (lane < p.buckets)
-            for (int i = 0; i < 64; ++i) sum += acc0[(wave * p.buckets + lane) * 64 + ((i + lane) & 63)].x;
-        float* const sums = reinterpret_cast<float*>(vec);             // (the vector, 390 words and more, has been read)
-        sums[wave * 64 + lane] = sum;
-        at_sync();
-        if (wave == 0) {
-            float all = sums[lane];
-            for (int w2 = 1; w2 < NW; ++w2) all += sums[w2 * 64 + lane];
-            part[lane] = all;
+        // lane b of each wave sums the wave's diagonals of bucket b, then one wave adds the waves
+#pragma unroll
+        for (int s = 32; s > 0; s >>= 1) {
+            farS[0] += __shfl_xor(farS[0], s, 64);
+            farS[1] += __shfl_xor(farS[1], s, 64);
         }
+        if (lane == 0) {
+            dvec[0] += farS[0];
+            dvec[2 * R] += farS[1];
+        }
+        float sum = 0.0f;
+        if (lane < p.buckets) {
+            const bool ahead = p.two_sided && lane >= p.side;          // r > 0
+            const int i = ahead ? lane - p.side : lane;
+            int lo = i < p.exact ? i : i == p.exact ? p.exact : p.border[i - p.exact - 1];           // distances lo .. hi
+            int hi = i < p.exact ? i : i - p.exact < p.nborder ? p.border[i - p.exact] - 1 : R;
+            if (ahead && lo == 0) lo = 1;                              // distance 0 is not ahead
+            for (int d = lo; d <= hi; ++d) sum += dvec[ahead ? R + d : R - d];
+            if (!p.two_sided && lane == 0)
+                for (int d = 1; d <= R; ++d) sum += dvec[R + d];       // one-sided: whatever is ahead counts as distance 0
+        }
+        at_sync();
+        skew0[wave * 64 + lane] = sum;
+        at_sync();
+        if (wave == 0) part[lane] = (skew0[lane] + skew0[64 + lane]) + (skew0[128 + lane] + skew0[192 + lane]);
     }
 }
 
@@ -917,11 +940,6 @@ int mi_launch_attention(hipStream_t st, mi_attn_args a, int dtype)
     return f16 ? launch_fwd<128, true>(st, a) : launch_fwd<128, false>(st, a);
 }
 
-// Blocks of the dQ kernel: four waves, or two where the table gradient's accumulators (512 bytes per bucket and wave) would leave
-// four waves no room beside the tiles.
-static int at_dq_waves(const mi_attn_args& a) { return a.table && a.buckets > 32 ? 2 : 4; }
-static int64_t at_dq_tiles(int64_t tokens, int64_t nseq, int BM) { return tokens / BM + nseq + 1; }
-
 // Shares of a group's query heads in the dK / dV kernel: the fewest that give AT_DKV_BLOCKS blocks (two per CU, four rounds, so
 // that a causal sequence's long first tiles even out), all heads at most.  1 x 8,191 causal, 8 heads on 2 key heads of 128:
 // 128 blocks 1,620 us, 512 blocks @DKV_SPLIT@ us.
@@ -939,20 +957,18 @@ size_t mi_attn_backward_bytes(const mi_attn_args& a)
     const size_t delta = mi_round_up((int64_t)a.heads * a.tokens * 4, 256);
     const int splits = at_dkv_splits(a);
     const size_t join = splits > 1 ? (size_t)mi_round_up((int64_t)splits * 2 * a.tokens * (a.heads / a.group) * a.hd * 4, 256) : 0;
-    const int64_t tiles = a.offsets ? at_dq_tiles(a.tokens, a.nseq, 32 * at_dq_waves(a))
-                                    : (int64_t)a.nseq * ((a.uniform_len + 32 * at_dq_waves(a) - 1) / (32 * at_dq_waves(a)));
+    const int64_t tiles = a.offsets ? a.tokens / 128 + a.nseq + 1 : (int64_t)a.nseq * ((a.uniform_len + 127) / 128);
     return delta + join + (a.table ? (size_t)(a.heads * tiles) * MI_ATTN_MAX_BUCKETS * 4 : 0);
 }
 
-template <int DP, bool F16, bool BIAS, int NW>
+template <int DP, bool F16, bool BIAS>
 static int launch_dq(hipStream_t st, mi_attn_args& a)
 {
-    const unsigned grid = at_schedule(&a, a.heads, 32 * NW);
+    const unsigned grid = at_schedule(&a, a.heads, 128);
     if (grid == 0) return MI_OK;
-    const int nvec = 2 * (a.reach + AT_PAD) + 1;
-    const size_t smem = 4 * AtTile<DP>::BYTES + (BIAS ? (size_t)NW * 2 * a.buckets * 64 * 4 + (size_t)nvec * 8 : 0);
-    MI_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(attn_dq_kernel<DP, F16, BIAS, NW>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    attn_dq_kernel<DP, F16, BIAS, NW><<<grid, 64 * NW, smem, st>>>(a);
+    const size_t smem = 4 * AtTile<DP>::BYTES + (BIAS ? (4 * 32 * 64 + 5 * (2 * (size_t)(a.reach + AT_PAD) + 1)) * 4 : 0);
+    MI_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(attn_dq_kernel<DP, F16, BIAS>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    attn_dq_kernel<DP, F16, BIAS><<<grid, 256, smem, st>>>(a);
     MI_HIP(hipGetLastError());
     return MI_OK;
 }
@@ -974,9 +990,8 @@ static int launch_bwd(hipStream_t st, mi_attn_args& a)
 {
     if (a.table) MI_TRY((launch_delta<DP, F16, true>(st, a)));
     else MI_TRY((launch_delta<DP, F16, false>(st, a)));
-    if (!a.table) MI_TRY((launch_dq<DP, F16, false, 4>(st, a)));
-    else if (at_dq_waves(a) == 4) MI_TRY((launch_dq<DP, F16, true, 4>(st, a)));
-    else MI_TRY((launch_dq<DP, F16, true, 2>(st, a)));
+    if (a.table) MI_TRY((launch_dq<DP, F16, true>(st, a)));
+    else MI_TRY((launch_dq<DP, F16, false>(st, a)));
     if (a.table) {
         attn_dtable_kernel<<<(unsigned)a.heads, 1024, 0, st>>>(a);
         MI_HIP(hipGetLastError());
