@@ -318,8 +318,8 @@ int  mi_encoder_last_time(const mi_encoder* enc, float* out_ms);
  * m + floor((n - m) log(d / m) / log(max_distance / m)), at most n - 1; borders that are whole numbers are exact.
  *
  * Tensors are given as rows of head_dim 16-bit elements: row (token t, head h) starts at ptr + t * token_stride +
- * h * head_stride (elements), its elements are adjacent.  ptr is 16-byte aligned, the strides are multiples of 8, head_dim is
- * a multiple of 8 up to 128.  Sequence i is rows offsets[i] .. offsets[i + 1] (device int32 [nseq + 1], rising from 0, at most
+ * h * head_stride (elements), its elements are adjacent.  ptr is 16-byte aligned, the strides are multiples of 8 (the token
+ * stride below 2^24), head_dim is a multiple of 8 up to 128.  Sequence i is rows offsets[i] .. offsets[i + 1] (device int32 [nseq + 1], rising from 0, at most
  * `tokens`; offsets outside that order give unspecified rows but no access outside the tensors); offsets = NULL: nseq
  * sequences of tokens / nseq rows each.  Sequences may be empty.  Rows behind the last sequence are left as they were, or, with
  * zero_tail, set to 0 (lse: -inf).  Values of one sequence never reach another, and rows that key_mask takes out may hold

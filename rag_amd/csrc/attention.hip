@@ -124,15 +124,17 @@ __device__ __forceinline__ bool at_find(const mi_attn_args& p, int t, int& start
 
 // ---------------------------------------------------------------- tiles in LDS
 // A tile is 64 rows of DP elements (head_dim rounded up to 32, 64 or 128), 16-byte chunks XOR-swizzled within the row so that both
-// reads are free of bank conflicts: 8 consecutive rows at one chunk (operand rows, ds_read_b128) and 4 consecutive rows at a
-// pair of chunks (the transpose read).  LDS-DMA writes lane i's 16 bytes at base + 16 i, so the swizzle is on the source side.
+// reads are free of bank conflicts (64 banks, 256 bytes a cycle): 16 consecutive rows at one chunk (operand rows, ds_read_b128) and
+// 4 consecutive rows at 4 chunks (the transpose read, 32 lanes).  LDS-DMA writes lane i's 16 bytes at base + 16 i, so the swizzle is on
+// the source side.
 template <int DP> struct AtTile {
     static constexpr int RP = DP * 2;                 // row pitch, bytes
     static constexpr int BYTES = AT_KT * RP;
     static __device__ __forceinline__ int f(int row)
     {
-        if constexpr (DP == 32) return (((row >> 1) & 1) << 1) | ((row >> 2) & 1);
-        else return ((row & 3) << 1) | ((row >> 2) & 1);
+        if constexpr (DP == 32) return (row >> 2) & 3;
+        else if constexpr (DP == 64) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+        else return ((row & 3) << 2) | ((row >> 2) & 3);
     }
 };
 
@@ -140,37 +142,50 @@ __device__ __forceinline__ void at_dma16(const void* src, unsigned lds_addr)
 {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(src), "s"(lds_addr) : "memory", "m0");
 }
+__device__ __forceinline__ void at_dma16(unsigned off, const char* base, unsigned lds_addr)
+{
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(off), "s"(base), "s"(lds_addr) : "memory", "m0");
+}
 
 // One operand's DMA: rows r0 .. r0 + 63 of a sequence (clamped to its last row) into the tile at lds_addr, by NW waves.
 // Chunks beyond head_dim repeat the last one: their products meet zeros of the other operand, or columns that are not stored.
 // Rows that the key mask takes out are staged as zeros: they may hold anything (0 x NaN in the product would not be 0).
+// A whole tile costs no vector instruction but the loads: scalar bases, one constant 32-bit lane offset (64 rows are below 2^31 bytes).
 __device__ const uint4 at_zero_chunk = {0, 0, 0, 0};
 template <int DP, int NW> struct AtStage {
-    const char* base;                                 // row 0 of the sequence, this lane's chunk
-    int64_t pitch;                                    // bytes between rows
-    int row0, last;                                   // this lane's row in instruction 0; the sequence's last row
+    static constexpr int LPR = DP / 8;                // lanes per row
+    static constexpr int RPI = 64 / LPR;              // rows per instruction
+    static constexpr int NI = AT_KT / (RPI * NW);
+    const char* base;                                 // row 0 of the sequence (uniform)
+    int pitch;                                        // bytes between rows
+    int row0, chunk;                                  // this lane's row in instruction 0 and its bytes in the row
+    unsigned off;
+    int last;                                         // the sequence's last row
     __device__ __forceinline__ void init(const mi_attn_rows& x, int start, int len, int head, int hd, int wave, int lane)
     {
-        constexpr int LPR = DP / 8;                   // lanes per row
-        const int lr = lane / LPR;
-        row0 = wave * (64 / LPR) + lr;
+        row0 = wave * RPI + lane / LPR;
         int c = (lane % LPR) ^ AtTile<DP>::f(row0);
         const int most = (hd >> 3) - 1;
-        c = c < most ? c : most;
-        base = reinterpret_cast<const char*>(x.p + (int64_t)start * x.ts + (int64_t)head * x.hs) + c * 16;
-        pitch = x.ts * 2;
+        chunk = (c < most ? c : most) * 16;
+        base = reinterpret_cast<const char*>(x.p + (int64_t)start * x.ts + (int64_t)head * x.hs);
+        pitch = (int)(x.ts * 2);
+        off = (unsigned)(row0 * pitch + chunk);
         last = len - 1;
     }
     __device__ __forceinline__ void issue(int r0, unsigned lds_addr, int wave, const int32_t* mask = nullptr) const
     {
-        constexpr int RPI = 64 / (DP / 8);            // rows per instruction
-        constexpr int NI = AT_KT / (RPI * NW);
+        const char* const at = base + (int64_t)r0 * pitch;
+        if (!mask && r0 + AT_KT - 1 <= last) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) at_dma16(off, at + (int64_t)i * RPI * NW * pitch, lds_addr + (unsigned)((i * NW + wave) * 1024));
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            int row = r0 + row0 + i * RPI * NW;
-            row = row < last ? row : last;
-            const char* src = base + (int64_t)row * pitch;
-            if (mask && mask[row] == 0) src = reinterpret_cast<const char*>(&at_zero_chunk);
+            int row = row0 + i * RPI * NW;
+            row = row < last - r0 ? row : last - r0;
+            const char* src = at + (int64_t)row * pitch + chunk;
+            if (mask && mask[r0 + row] == 0) src = reinterpret_cast<const char*>(&at_zero_chunk);
             at_dma16(src, lds_addr + (unsigned)((i * NW + wave) * 1024));
         }
     }
@@ -208,11 +223,11 @@ __device__ __forceinline__ u32x4 at_rows(const char* tile, int st, int s, int co
 template <int DP>
 __device__ __forceinline__ u32x4 at_cols(const char* tile, int ks, int dt, int lane)
 {
-    const int half = lane >> 5, r = 16 * ks + 4 * half + ((lane & 15) >> 2);
+    const int r = 4 * (lane >> 5) + ((lane & 15) >> 2);                // + 16 ks (+ 8: f differs)
     const int c = 4 * dt + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-    const char* a = tile + r * AtTile<DP>::RP + ((c ^ AtTile<DP>::f(4 * half + ((lane & 15) >> 2))) << 4) + 8 * (lane & 1);
-    const tr4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr4_lds_t*)(a));
-    const tr4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr4_lds_t*)(a + 8 * AtTile<DP>::RP));
+    const char* const a = tile + (16 * ks + r) * AtTile<DP>::RP + 8 * (lane & 1);
+    const tr4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr4_lds_t*)(a + ((c ^ AtTile<DP>::f(r)) << 4)));
+    const tr4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr4_lds_t*)(a + ((c ^ AtTile<DP>::f(r + 8)) << 4) + 8 * AtTile<DP>::RP));
     return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 // DP columns of one row from transposed accumulators (column 32 dt + 8 g + 4 half + i), times f, as 16-bit elements
@@ -304,7 +319,7 @@ __device__ __forceinline__ uint32_t at_allowed(const mi_attn_args& p, uint64_t k
 // barrier per tile.  The running maximum is an exponent reference that only has to keep exp2 in range: it moves, and O and l are
 // rescaled, when a tile's maximum exceeds it by more than 2^8.
 template <int DP, bool F16, bool BIAS, int QB>
-__global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const mi_attn_args p)
+__global__ __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) void attn_fwd_kernel(const mi_attn_args p)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     constexpr int BM = 128 * QB, TB = AtTile<DP>::BYTES;
@@ -1059,6 +1074,7 @@ static int fill_rows(const char* who, const char* what, const mi_attention_rows*
     MI_REQUIRE(((uintptr_t)r->ptr & 15) == 0, "%s: %s is not 16-byte aligned", who, what);
     MI_REQUIRE(r->token_stride % 8 == 0 && r->head_stride % 8 == 0, "%s: strides of %s (%lld, %lld) must be multiples of 8 elements", who, what,
                (long long)r->token_stride, (long long)r->head_stride);
+    MI_REQUIRE(r->token_stride < ((int64_t)1 << 24), "%s: token stride of %s, %lld, is not below 2^24 elements", who, what, (long long)r->token_stride);
     MI_REQUIRE(r->token_stride >= 0 && r->head_stride >= 0 && (tokens <= 1 || r->token_stride >= hd) && (heads <= 1 || r->head_stride >= hd),
                "%s: strides of %s (%lld, %lld) let rows of %d elements overlap", who, what, (long long)r->token_stride, (long long)r->head_stride, hd);
     out->p = (uint16_t*)r->ptr;

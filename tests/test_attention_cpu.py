@@ -93,6 +93,7 @@ BAD = [
     (dict(rows=dict(k=(0, (1 << 20) + 8))), "k is not 16-byte aligned"),
     (dict(rows=dict(v=(1, 132))), "strides of v"),
     (dict(rows=dict(out=(2, 68))), "strides of out"),
+    (dict(rows=dict(v=(1, 1 << 24))), "2^24"),
     (dict(rows=dict(q=(1, 56))), "overlap"),
     (dict(rows=dict(k=(2, 0))), "overlap"),
     (dict(rows=dict(q=(1, -256))), "overlap"),
