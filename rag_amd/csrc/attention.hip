@@ -8,7 +8,7 @@
 // read with the same permutation of keys by the hardware transpose read, so no value crosses a lane).
 #include <float.h>
 #include <math.h>
-#include <mutex>
+#include <atomic>
 #include "attention.h"
 #include "kernels.h"
 
@@ -929,6 +929,21 @@ static unsigned at_schedule(mi_attn_args* a, int heads, int BM)
     return (unsigned)((int64_t)heads * a->parts * a->tiles_per_unit);
 }
 
+// Leave for more than the default 64 KB of dynamic LDS, asked for once per kernel and device.
+template <auto KERNEL>
+static int at_lds(size_t bytes)
+{
+    static std::atomic<uint64_t> done{0};
+    if (bytes <= 64 * 1024) return MI_OK;
+    int dev = 0;
+    MI_HIP(hipGetDevice(&dev));
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return MI_OK;
+    MI_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+    if (dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+    return MI_OK;
+}
+
 template <int DP, bool F16>
 static int launch_fwd(hipStream_t st, mi_attn_args& a)
 {
@@ -937,10 +952,10 @@ static int launch_fwd(hipStream_t st, mi_attn_args& a)
     if (grid == 0) return MI_OK;
     if (a.table) {
         smem += (2 * (size_t)(a.reach + AT_PAD) + 1) * sizeof(float);
-        MI_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(attn_fwd_kernel<DP, F16, true, 1>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        MI_TRY((at_lds<&attn_fwd_kernel<DP, F16, true, 1>>(smem)));
         attn_fwd_kernel<DP, F16, true, 1><<<grid, 256, smem, st>>>(a);
     } else {
-        MI_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(attn_fwd_kernel<DP, F16, false, 1>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        MI_TRY((at_lds<&attn_fwd_kernel<DP, F16, false, 1>>(smem)));
         attn_fwd_kernel<DP, F16, false, 1><<<grid, 256, smem, st>>>(a);
     }
     MI_HIP(hipGetLastError());
@@ -982,7 +997,7 @@ static int launch_dq(hipStream_t st, mi_attn_args& a)
     const unsigned grid = at_schedule(&a, a.heads, 128);
     if (grid == 0) return MI_OK;
     const size_t smem = 4 * AtTile<DP>::BYTES + (BIAS ? (4 * 32 * 64 + 5 * (2 * (size_t)(a.reach + AT_PAD) + 1)) * 4 : 0);
-    MI_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(attn_dq_kernel<DP, F16, BIAS>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    MI_TRY((at_lds<&attn_dq_kernel<DP, F16, BIAS>>(smem)));
     attn_dq_kernel<DP, F16, BIAS><<<grid, 256, smem, st>>>(a);
     MI_HIP(hipGetLastError());
     return MI_OK;
@@ -994,7 +1009,7 @@ static int launch_delta(hipStream_t st, mi_attn_args& a)
     const unsigned grid = at_schedule(&a, a.heads, 128);
     if (grid == 0) return MI_OK;
     const size_t smem = 4 * AtTile<DP>::BYTES + (BIAS ? (size_t)(2 * (a.reach + AT_PAD) + 1) * 4 : 0);
-    MI_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(attn_delta_kernel<DP, F16, BIAS>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    MI_TRY((at_lds<&attn_delta_kernel<DP, F16, BIAS>>(smem)));
     attn_delta_kernel<DP, F16, BIAS><<<grid, 256, smem, st>>>(a);
     MI_HIP(hipGetLastError());
     return MI_OK;
@@ -1015,10 +1030,10 @@ static int launch_bwd(hipStream_t st, mi_attn_args& a)
     if (grid == 0) return MI_OK;
     const size_t smem = 4 * AtTile<DP>::BYTES + 1024 + (a.table ? (size_t)(2 * (a.reach + AT_PAD) + 1) * 4 : 0);
     if (a.table) {
-        MI_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(attn_dkv_kernel<DP, F16, true>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        MI_TRY((at_lds<&attn_dkv_kernel<DP, F16, true>>(smem)));
         attn_dkv_kernel<DP, F16, true><<<grid, 256, smem, st>>>(a);
     } else {
-        MI_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(attn_dkv_kernel<DP, F16, false>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        MI_TRY((at_lds<&attn_dkv_kernel<DP, F16, false>>(smem)));
         attn_dkv_kernel<DP, F16, false><<<grid, 256, smem, st>>>(a);
     }
     MI_HIP(hipGetLastError());
