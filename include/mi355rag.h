@@ -332,7 +332,7 @@ typedef struct {
     int32_t dtype;                    /* MI_DTYPE_BF16 or MI_DTYPE_F16 */
     int32_t causal;
     int32_t zero_tail;
-    float   scale;                    /* > 0 */
+    float   scale;                    /* 1e-20 .. 1e20 */
     int32_t num_buckets;              /* 0: no bias; else 2 (bidirectional: 4, even) .. 64 */
     int32_t max_distance;             /* above the exact buckets' distances, at most 1024 */
     int32_t bidirectional;

@@ -8,6 +8,7 @@
 // read with the same permutation of keys by the hardware transpose read, so no value crosses a lane).
 #include <float.h>
 #include <math.h>
+#include <stdlib.h>
 #include <atomic>
 #include "attention.h"
 #include "kernels.h"
@@ -71,14 +72,16 @@ __device__ __forceinline__ f32x16 at_zero16()
 // Blocks go to the 8 XCDs round robin by their linear id, and each XCD has its own L2.  A unit is a head, or, where the heads
 // are no multiple of 8, every parts-th tile of a head; an XCD owns units_per_xcd consecutive units, so the query heads of one key
 // head read its K and V through one L2, and every XCD has the same mix of tiles (a causal sequence's last tiles are its longest).
+// Grid: x = 8 XCDs x a unit's tiles, y = the XCD's units, so nothing is divided.
 __device__ __forceinline__ bool at_work(const mi_attn_args& p, int& head, int& t)
 {
-    const int xcd = blockIdx.x & 7, idx = blockIdx.x >> 3;
-    const int u = xcd * p.units_per_xcd + idx / p.tiles_per_unit;
-    head = u / p.parts;
-    t = (idx % p.tiles_per_unit) * p.parts + u % p.parts;
+    const int u = (blockIdx.x & 7) * p.units_per_xcd + blockIdx.y;
+    head = u >> p.parts_log2;
+    t = ((blockIdx.x >> 3) << p.parts_log2) + (u & ((1 << p.parts_log2) - 1));
     return t < p.tiles;
 }
+// x / d for x < 2^16 and m = ceil(2^32 / d)
+__device__ __forceinline__ int at_div(int x, uint32_t m) { return m ? (int)__umulhi((uint32_t)x, m) : x; }
 
 // Tile t of the token axis -> sequence and tile of it.  Tiles of sequence i start at offsets[i] / BM + i: an upper bound of the
 // tiles before it that needs no prefix sum; the surplus finds no rows.  64 lanes probe 64 sequences at a time.  With zero_tail
@@ -138,9 +141,20 @@ template <int DP> struct AtTile {
     }
 };
 
+// A pointer that is the same on every lane, in scalar registers (hipcc may have moved it to vector ones)
+__device__ __forceinline__ const char* at_uniform(const char* x)
+{
+    const uint64_t u = (uint64_t)x;
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)u), hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(u >> 32));
+    return (const char*)((uint64_t)hi << 32 | lo);
+}
 __device__ __forceinline__ void at_dma16(const void* src, unsigned lds_addr)
 {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(src), "s"(lds_addr) : "memory", "m0");
+}
+__device__ __forceinline__ void at_dma4(const void* src, unsigned lds_addr)
+{
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" :: "v"(src), "s"(lds_addr) : "memory", "m0");
 }
 __device__ __forceinline__ void at_dma16(unsigned off, const char* base, unsigned lds_addr)
 {
@@ -156,38 +170,88 @@ template <int DP, int NW> struct AtStage {
     static constexpr int LPR = DP / 8;                // lanes per row
     static constexpr int RPI = 64 / LPR;              // rows per instruction
     static constexpr int NI = AT_KT / (RPI * NW);
-    const char* base;                                 // row 0 of the sequence (uniform)
+    const char* at;                                   // the next tile's row 0 (uniform): tiles are requested in order
     int pitch;                                        // bytes between rows
     int row0, chunk;                                  // this lane's row in instruction 0 and its bytes in the row
     unsigned off;
-    int last;                                         // the sequence's last row
-    __device__ __forceinline__ void init(const mi_attn_rows& x, int start, int len, int head, int hd, int wave, int lane)
+    int left;                                         // rows from `at` to the sequence's last one
+    __device__ __forceinline__ void init(const mi_attn_rows& x, int start, int first, int len, int head, int hd, int wave, int lane)
     {
         row0 = wave * RPI + lane / LPR;
         int c = (lane % LPR) ^ AtTile<DP>::f(row0);
         const int most = (hd >> 3) - 1;
         chunk = (c < most ? c : most) * 16;
-        base = reinterpret_cast<const char*>(x.p + (int64_t)start * x.ts + (int64_t)head * x.hs);
-        pitch = (int)(x.ts * 2);
+        at = at_uniform(reinterpret_cast<const char*>(x.p + (int64_t)(start + first) * x.ts + (int64_t)head * x.hs));
+        pitch = __builtin_amdgcn_readfirstlane((int)(x.ts * 2));
         off = (unsigned)(row0 * pitch + chunk);
-        last = len - 1;
+        left = len - 1 - first;
     }
-    __device__ __forceinline__ void issue(int r0, unsigned lds_addr, int wave, const int32_t* mask = nullptr) const
+    // the next 64 rows to lds_addr; mask: the key mask from the tile's first row on
+    __device__ __forceinline__ void issue(unsigned lds_addr, int wave, const int32_t* mask = nullptr)
     {
-        const char* const at = base + (int64_t)r0 * pitch;
-        if (!mask && r0 + AT_KT - 1 <= last) {
+        lds_addr += wave * 1024;
+        if (!mask && left >= AT_KT - 1) {
 #pragma unroll
-            for (int i = 0; i < NI; ++i) at_dma16(off, at + (int64_t)i * RPI * NW * pitch, lds_addr + (unsigned)((i * NW + wave) * 1024));
-            return;
-        }
+            for (int i = 0; i < NI; ++i) {
+                at_dma16(off, at, lds_addr + (unsigned)(i * NW * 1024));
+                at += RPI * NW * pitch;               // (below 2^31)
+            }
+        } else {
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            int row = row0 + i * RPI * NW;
-            row = row < last - r0 ? row : last - r0;
-            const char* src = at + (int64_t)row * pitch + chunk;
-            if (mask && mask[r0 + row] == 0) src = reinterpret_cast<const char*>(&at_zero_chunk);
-            at_dma16(src, lds_addr + (unsigned)((i * NW + wave) * 1024));
+            for (int i = 0; i < NI; ++i) {
+                int row = row0 + i * RPI * NW;
+                row = row < left ? row : left;
+                const char* src = at + (int64_t)row * pitch + chunk;
+                if (mask && mask[row] == 0) src = reinterpret_cast<const char*>(&at_zero_chunk);
+                at_dma16(src, lds_addr + (unsigned)(i * NW * 1024));
+            }
+            at += (int64_t)AT_KT * pitch;
         }
+        left -= AT_KT;
+    }
+};
+// Everything a wave issued but its last AHEAD x PER loads has landed and what it read from LDS is in registers, on every wave.
+template <int PER>
+__device__ __forceinline__ void at_arrive(int ahead)
+{
+    if (ahead >= 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * PER) : "memory");
+    else if (ahead == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(PER) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+// The K and V tiles of a sequence through NB pairs of buffers: tile t + NB - 1 is requested when every wave is done with tile t - 1.
+// (With two buffers a tile has one tile's computing to arrive, about 0.5 us at head size 32, and memory takes longer.)
+template <int DP, int NB> struct AtPipe {
+    static constexpr int PAIR = 2 * AtTile<DP>::BYTES, BYTES = NB * PAIR, PER = 2 * AtStage<DP, 4>::NI;
+    AtStage<DP, 4> a, b;
+    const int32_t* mask;
+    unsigned lds0;
+    int n, wave, buf;
+    __device__ __forceinline__ void issue(int t, int slot)
+    {
+        const int32_t* const m = mask ? mask + t * AT_KT : nullptr;
+        a.issue(lds0 + slot * PAIR, wave, m);
+        b.issue(lds0 + slot * PAIR + PAIR / 2, wave, m);
+    }
+    __device__ __forceinline__ void start(const char* lds, int tiles, const int32_t* key_mask, int w)
+    {
+        lds0 = (unsigned)(size_t)(const __attribute__((address_space(3))) char*)lds;
+        n = tiles;
+        mask = key_mask;
+        wave = w;
+        buf = NB - 1;
+#pragma unroll
+        for (int t = 0; t < NB - 1; ++t) if (t < n) issue(t, t);
+    }
+    // tile t has landed; returns its place
+    __device__ __forceinline__ int next(int t)
+    {
+        const int left = n - 1 - t;
+        at_arrive<PER>(left < NB - 2 ? left : NB - 2);
+        if (t + NB - 1 < n) issue(t + NB - 1, buf);                    // over tile t - 1
+        buf = buf + 1 == NB ? 0 : buf + 1;
+        return buf * PAIR;
     }
 };
 // everything outstanding has landed and been read, on every wave
@@ -269,7 +333,8 @@ __device__ __forceinline__ void at_zero_rows(const mi_attn_rows& x, int64_t toke
 
 // ---------------------------------------------------------------- relative position bias
 // In LDS as a vector over r = key - query, [-(reach + AT_PAD), reach + AT_PAD]: a 64 x 32 tile of scores that touches |r| < reach
-// stays inside it, any other tile lies in one bucket.  Values are in log2 units.
+// stays inside it, any other tile lies in one bucket.  Values are times `unit`: log2(e), to be added to scaled scores, or 1 / scale, to be
+// the C operand of a score block's first product.
 // A finite bias counts as at most 4096 in size.  Beyond that it only says "never" or "always" (exp(-4096) is 0 beside any other
 // score), and a running reference near the type's lowest value would swallow the scores of the keys that come after it; at 4096
 // fp32 still resolves a score to 2^-12, half of fp16's step in p.
@@ -281,19 +346,21 @@ __host__ __device__ __forceinline__ int at_bucket(const mi_attn_args& p, int r)
     int b = d;
     if (d >= p.exact) {
         b = p.exact;
-        for (int t = 0; t < p.nborder; ++t) b += d >= p.border[t] ? 1 : 0;
+        for (int t = 0; t < p.nborder; t += 8)                         // (the array ends in values beyond any distance)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) b += d >= p.border[t + j] ? 1 : 0;
     }
     return b + (p.two_sided && r > 0 ? p.side : 0);
 }
-__device__ __forceinline__ float at_bias(const mi_attn_args& p, int head, int r)
+__device__ __forceinline__ float at_bias(const mi_attn_args& p, int head, int r, float unit)
 {
     const float x = p.table[(int64_t)at_bucket(p, r) * p.heads + head];
-    return (fabsf(x) <= FLT_MAX ? fminf(fmaxf(x, -AT_BIAS_MOST), AT_BIAS_MOST) : x) * AT_LOG2E;
+    return (fabsf(x) <= FLT_MAX ? fminf(fmaxf(x, -AT_BIAS_MOST), AT_BIAS_MOST) : x) * unit;
 }
-__device__ __forceinline__ void at_fill_bias(const mi_attn_args& p, int head, float* vec)
+__device__ __forceinline__ void at_fill_bias(const mi_attn_args& p, int head, float unit, float* vec)
 {
     const int R = p.reach + AT_PAD;
-    for (int i = threadIdx.x; i < 2 * R + 1; i += blockDim.x) vec[i] = at_bias(p, head, i - R);
+    for (int i = threadIdx.x; i < 2 * R + 1; i += blockDim.x) vec[i] = at_bias(p, head, i - R, unit);
 }
 
 // Which of the 64 keys at k0 are keys of the sequence that the mask leaves (bit = key - k0); the wave's lanes ask for one each.
@@ -314,16 +381,31 @@ __device__ __forceinline__ uint32_t at_allowed(const mi_attn_args& p, uint64_t k
     return ok >> (4 * half);
 }
 
+// The first of a score block's products, on the bias where it is not one value for the tile: 8 g + i steps on from bv
+template <bool F16>
+__device__ __forceinline__ f32x16 at_first(bool near, const float* bv, int step, u32x4 a, u32x4 b)
+{
+    if (near) {
+        f32x16 C;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) C[i] = bv[step * (8 * (i >> 2) + (i & 3))];
+        return at_mfma<F16>(a, b, C);
+    }
+    return at_mfma<F16>(a, b, at_zero16());
+}
+
 // ---------------------------------------------------------------- forward
-// One block per (head, 128 QB query rows), four waves of 32 QB queries; K and V tiles of 64 keys by LDS-DMA, double-buffered, one
-// barrier per tile.  The running maximum is an exponent reference that only has to keep exp2 in range: it moves, and O and l are
-// rescaled, when a tile's maximum exceeds it by more than 2^8.
-template <int DP, bool F16, bool BIAS, int QB>
+#define AT_BUFFERS(DP) ((DP) == 32 ? 4 : (DP) == 64 ? 3 : 2)          // what leaves LDS for as many blocks as the registers do
+// One block per (head, 128 / KS query rows): four waves, each 32 queries by every KS-th 32-key block of the K and V tiles, which come by
+// LDS-DMA, 64 keys at a time, one barrier per tile.  The running maximum is an exponent reference that only has to keep exp2 in
+// range: it moves, and O and l are rescaled, when a tile's maximum exceeds it by more than 2^8 (fp16: 2^15).  With KS = 2 the two
+// waves of a query join their sums through LDS at the end: half the time per tile and twice the blocks, for calls of few blocks.
+template <int DP, bool F16, bool BIAS, int KS>
 __global__ __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) void attn_fwd_kernel(const mi_attn_args p)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    constexpr int BM = 128 * QB, TB = AtTile<DP>::BYTES;
-    float* const vec = reinterpret_cast<float*>(lds + 4 * TB);
+    constexpr int BM = 128 / KS, TB = AtTile<DP>::BYTES, NS = 2 / KS, NB = AT_BUFFERS(DP);
+    float* const vec = reinterpret_cast<float*>(lds + NB * 2 * TB);
     int head, t, start, len, tile;
     bool tail;
     if (!at_work(p, head, t) || !at_find<BM>(p, t, start, len, tile, tail)) return;
@@ -336,147 +418,142 @@ __global__ __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) void attn_fwd
         return;
     }
     if (p.causal) tile = (len + BM - 1) / BM - 1 - tile;               // the longest rows first
-    const int qw = tile * BM + wave * 32 * QB;                         // this wave's first query
+    const int qw = tile * BM + (KS == 1 ? wave : wave & 1) * 32, q = qw + col;   // this wave's queries
+    const int s0 = KS == 1 ? 0 : wave >> 1;                            // its first 32-key block of a tile
     const int kend = p.causal ? (tile * BM + BM < len ? tile * BM + BM : len) : len;
 
-    u32x4 qf[QB][DP / 16];
-#pragma unroll
-    for (int b = 0; b < QB; ++b) {
-        const int q = qw + 32 * b + col;
-        at_load_rows<DP>(qf[b], p.q, start + (q < len ? q : len - 1), head, p.hd, half);
-    }
-    const int kvh = head / p.group;
-    AtStage<DP, 4> ks, vs;
-    ks.init(p.k, start, len, kvh, p.hd, wave, lane);
-    vs.init(p.v, start, len, kvh, p.hd, wave, lane);
-    const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds;
+    u32x4 qf[DP / 16];
+    at_load_rows<DP>(qf, p.q, start + (q < len ? q : len - 1), head, p.hd, half);
+    const int kvh = at_div(head, p.group_inv);
     const int32_t* const mask = p.key_mask ? p.key_mask + start : nullptr;
-    ks.issue(0, lds0, wave, mask);
-    vs.issue(0, lds0 + TB, wave, mask);
-    if constexpr (BIAS) at_fill_bias(p, head, vec);
+    AtPipe<DP, NB> pipe;
+    pipe.a.init(p.k, start, 0, len, kvh, p.hd, wave, lane);
+    pipe.b.init(p.v, start, 0, len, kvh, p.hd, wave, lane);
+    pipe.start(lds, (kend + AT_KT - 1) / AT_KT, mask, wave);
+    if constexpr (BIAS) at_fill_bias(p, head, AT_LOG2E, vec);
 
-    f32x16 O[QB][DP / 32];
-    float m[QB], thr[QB], l[QB];
+    f32x16 O[DP / 32];
 #pragma unroll
-    for (int b = 0; b < QB; ++b) {
-#pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt) O[b][dt] = at_zero16();
-        m[b] = 0.0f;
-        thr[b] = -INFINITY;                                            // no finite score seen yet
-        l[b] = 0.0f;
-    }
+    for (int dt = 0; dt < DP / 32; ++dt) O[dt] = at_zero16();
+    // the reference starts at a usual place and stays while the first tile's maximum lies within 2^8 of it; bf16 has fp32's range,
+    // fp16 takes it 2^8 lower so that the sum is at least 1, and p up to 2^15
+    constexpr float M0 = F16 ? -8.0f : 0.0f, HIGH = F16 ? 15.0f : 8.0f, LOW = F16 ? 0.0f : -8.0f;
+    float m = M0, low = LOW, l = 0.0f;                                 // low = -inf once a finite score has been seen
     const int R = p.reach + AT_PAD;
-    for (int k0 = 0, buf = 0; k0 < kend; k0 += AT_KT, buf ^= 1) {
-        at_sync();                                                     // this tile has landed, the other buffer has been read
-        if (k0 + AT_KT < kend) {
-            ks.issue(k0 + AT_KT, lds0 + (buf ^ 1) * 2 * TB, wave, mask);
-            vs.issue(k0 + AT_KT, lds0 + (buf ^ 1) * 2 * TB + TB, wave, mask);
-        }
-        if (qw >= len || (p.causal && k0 > qw + 32 * QB - 1)) continue;  // nothing for this wave (it has met the barrier)
-        const char* const Kt = lds + buf * 2 * TB;
+    const float c = p.scale_log2;
+    for (int k0 = 0; k0 < kend; k0 += AT_KT) {
+        const char* const Kt = lds + pipe.next(k0 / AT_KT);
         const char* const Vt = Kt + TB;
+        // nothing for this wave (it has met the barrier)
+        const int kw = k0 + 32 * s0;
+        if (qw >= len || kw >= kend || (p.causal && kw > qw + 31)) continue;
         const uint64_t keys = at_keys(mask, k0, len, lane);
-        const bool masked = ~keys != 0 || (p.causal && k0 + AT_KT - 1 > qw);
+        const bool masked = ~keys != 0 || (p.causal && kw + 32 * NS - 1 > qw);
 
-        f32x16 S[QB][2];
-#pragma unroll
-        for (int st = 0; st < 2; ++st)
-#pragma unroll
-            for (int s = 0; s < DP / 16; ++s) {
-                const u32x4 kf = at_rows<DP>(Kt, st, s, col, half);
-#pragma unroll
-                for (int b = 0; b < QB; ++b) S[b][st] = at_mfma<F16>(kf, qf[b][s], s == 0 ? at_zero16() : S[b][st]);
-            }
-#pragma unroll
-        for (int b = 0; b < QB; ++b) {
-            const int q = qw + 32 * b + col;
-            const float c = p.scale_log2;
-            // x = score in log2 units, less the reference
-            if constexpr (BIAS) {
-                const int rlo = k0 - (qw + 32 * b + 31), rhi = k0 + AT_KT - 1 - (qw + 32 * b);
-                if (rhi <= -p.reach || rlo >= p.reach) {
-                    const float far = vec[rhi <= -p.reach ? 0 : 2 * R] - m[b];
-#pragma unroll
-                    for (int st = 0; st < 2; ++st)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) S[b][st][i] = __builtin_fmaf(S[b][st][i], c, far);
-                } else {
-                    const float* bv = vec + (k0 + 4 * half - q + R);
-#pragma unroll
-                    for (int st = 0; st < 2; ++st)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            S[b][st][i] = __builtin_fmaf(S[b][st][i], c, bv[32 * st + 8 * (i >> 2) + (i & 3)] - m[b]);
-                }
-            } else {
-#pragma unroll
-                for (int st = 0; st < 2; ++st)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) S[b][st][i] = __builtin_fmaf(S[b][st][i], c, -m[b]);
-            }
-            if (masked) {
-#pragma unroll
-                for (int st = 0; st < 2; ++st) {
-                    const uint32_t ok = at_allowed(p, keys, st, q - k0, half);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) S[b][st][i] = (ok >> (8 * (i >> 2) + (i & 3))) & 1u ? S[b][st][i] : -INFINITY;
-                }
-            }
-            float top = S[b][0][0];
-#pragma unroll
-            for (int i = 1; i < 15; i += 2) top = at_max3(top, S[b][0][i], S[b][0][i + 1]);
-            top = at_max3(top, S[b][0][15], S[b][1][0]);
-#pragma unroll
-            for (int i = 1; i < 15; i += 2) top = at_max3(top, S[b][1][i], S[b][1][i + 1]);
-            top = fmaxf(top, S[b][1][15]);
-            if (__builtin_amdgcn_ballot_w64(top > thr[b]) != 0) {
-                top = fmaxf(top, at_other_half(top));                  // both halves of a query move alike
-                const bool move = top > thr[b];
-                const float up = move ? top : 0.0f;
-                const float alpha = move ? (thr[b] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-up)) : 1.0f;
-                m[b] += up;
-                if (move) thr[b] = 8.0f;
-                l[b] *= alpha;
-#pragma unroll
-                for (int dt = 0; dt < DP / 32; ++dt) O[b][dt] = O[b][dt] * alpha;
-#pragma unroll
-                for (int st = 0; st < 2; ++st)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) S[b][st][i] -= up;
-            }
-#pragma unroll
-            for (int st = 0; st < 2; ++st)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    S[b][st][i] = __builtin_amdgcn_exp2f(S[b][st][i]);
-                    l[b] += S[b][st][i];
-                }
+        f32x16 S[NS];
+        float less = -m;                                               // what is left to add to c S
+        bool near = false;
+        const float* bv = vec;
+        if constexpr (BIAS) {
+            const int rlo = kw - (qw + 31), rhi = kw + 32 * NS - 1 - qw;
+            near = rhi > -p.reach && rlo < p.reach;
+            bv = vec + (kw + 4 * half - q + R);
+            if (!near) less += vec[rhi <= -p.reach ? 0 : 2 * R];
         }
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-            u32x4 pf[QB];
+        for (int n = 0; n < NS; ++n)
 #pragma unroll
-            for (int b = 0; b < QB; ++b)
+            for (int s = 0; s < DP / 16; ++s) S[n] = at_mfma<F16>(at_rows<DP>(Kt, s0 + n, s, col, half), qf[s], s == 0 ? at_zero16() : S[n]);
+        // score in log2 units, less the reference
+        if (near) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    pf[b][i] = at_pack2<F16>(S[b][kk >> 1][8 * (kk & 1) + 2 * i], S[b][kk >> 1][8 * (kk & 1) + 2 * i + 1]);
+            for (int n = 0; n < NS; ++n)
 #pragma unroll
-            for (int dt = 0; dt < DP / 32; ++dt) {
-                const u32x4 vf = at_cols<DP>(Vt, kk, dt, lane);
+                for (int i = 0; i < 16; ++i) S[n][i] = __builtin_fmaf(S[n][i], c, bv[32 * n + 8 * (i >> 2) + (i & 3)] - m);
+        } else {
 #pragma unroll
-                for (int b = 0; b < QB; ++b) O[b][dt] = at_mfma<F16>(vf, pf[b], O[b][dt]);
+            for (int n = 0; n < NS; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) S[n][i] = __builtin_fmaf(S[n][i], c, less);
+        }
+        if (masked) {
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+                const uint32_t ok = at_allowed(p, keys, s0 + n, q - k0, half);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) S[n][i] = (ok >> (8 * (i >> 2) + (i & 3))) & 1u ? S[n][i] : -INFINITY;
             }
+        }
+        float top = S[0][0];
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+            for (int i = n == 0 ? 1 : 0; i + 1 < 16; i += 2) top = at_max3(top, S[n][i], S[n][i + 1]);
+        top = fmaxf(top, S[0][15]);
+        if (__builtin_amdgcn_ballot_w64(top > HIGH || top < low) != 0) {
+            top = fmaxf(top, at_other_half(top));                      // both halves of a query move alike
+            low = fminf(low, at_other_half(low));
+            const bool move = top > HIGH || (top < low && top > -INFINITY);
+            const float up = move ? top : 0.0f;
+            const float alpha = low > -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(-up);   // (nothing summed before the first)
+            m += up;
+            l *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; ++dt) O[dt] = O[dt] * alpha;
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) S[n][i] -= up;
+        }
+        low = top > -INFINITY ? -INFINITY : low;
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                S[n][i] = __builtin_amdgcn_exp2f(S[n][i]);
+                l += S[n][i];
+            }
+#pragma unroll
+        for (int kk = 0; kk < 2 * NS; ++kk) {
+            u32x4 pf;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) pf[i] = at_pack2<F16>(S[kk >> 1][8 * (kk & 1) + 2 * i], S[kk >> 1][8 * (kk & 1) + 2 * i + 1]);
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; ++dt) O[dt] = at_mfma<F16>(at_cols<DP>(Vt, 2 * s0 + kk, dt, lane), pf, O[dt]);
         }
     }
+    float sum = l + at_other_half(l);
+    if constexpr (KS == 2) {
+        // waves 2 and 3 hand over reference, sum and O; rows of 64 lanes, one register each
+        low = fminf(low, at_other_half(low));
+        at_sync();
+        float* const x = reinterpret_cast<float*>(lds) + (wave & 1) * (DP / 2 + 3) * 64 + lane;
+        if (wave >= 2) {
+            x[0] = m;
+            x[64] = sum;
+            x[128] = low;
 #pragma unroll
-    for (int b = 0; b < QB; ++b) {
-        const int q = qw + 32 * b + col;
-        const float sum = l[b] + at_other_half(l[b]);
-        if (q < len) {
-            at_store_row<DP, F16>(p.out, start + q, head, p.hd, half, O[b], sum == 0.0f ? 0.0f : 1.0f / sum);
-            if (p.lse && half == 0)
-                p.lse[(int64_t)head * p.tokens + start + q] = sum == 0.0f ? -INFINITY : (m[b] + __builtin_amdgcn_logf(sum)) * AT_LN2;
+            for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[(3 + 16 * dt + i) * 64] = O[dt][i];
         }
+        at_sync();
+        if (wave >= 2) return;
+        const float m2 = x[0], sum2 = x[64], low2 = x[128];
+        // a side without a finite score has summed nothing (or NaN): the other side's reference stands
+        const float mm = low > -INFINITY ? m2 : low2 > -INFINITY ? m : fmaxf(m, m2);
+        const float f1 = low > -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mm), f2 = low2 > -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m2 - mm);
+        m = mm;
+        sum = sum * f1 + sum2 * f2;
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) O[dt][i] = O[dt][i] * f1 + x[(3 + 16 * dt + i) * 64] * f2;
+    }
+    if (q < len) {
+        at_store_row<DP, F16>(p.out, start + q, head, p.hd, half, O, sum == 0.0f ? 0.0f : 1.0f / sum);
+        if (p.lse && half == 0)
+            p.lse[(int64_t)head * p.tokens + start + q] = sum == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * AT_LN2;
     }
 }
 
@@ -488,13 +565,14 @@ template <bool F16> struct AtPScale { static constexpr float log2 = F16 ? 12.0f 
 // D = sum_j p dp of every row.  rowsum(dout * out) is the same sum, but takes over the rounding of p and out in the forward pass,
 // which shows in rows of few keys (20 causal rows: dq and dk 1.65 x the plain rounding of their values, 1.4 with D exact) and in
 // the table's gradient, a sum of many ds that nearly cancel.  So with a bias, for rows of up to 128 keys, and for up to 512 where
-// a mask may leave few of them, the sum is made from the scores, in fp32; other rows take the dot product.
+// a mask may leave few of them, the sum is made from the scores, in fp32; other rows take the dot product.  Also writes the rows'
+// log-sum-exp the way the other two kernels take it: in log2 units, +inf for a row that attends nothing.
 template <int DP, bool F16, bool BIAS>
 __global__ __launch_bounds__(256, 2) void attn_delta_kernel(const mi_attn_args p)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    constexpr int BM = 128, TB = AtTile<DP>::BYTES;
-    float* const vec = reinterpret_cast<float*>(lds + 4 * TB);
+    constexpr int BM = 128, TB = AtTile<DP>::BYTES, NB = AT_BUFFERS(DP);
+    float* const vec = reinterpret_cast<float*>(lds + NB * 2 * TB);
     int head, t, start, len, tile;
     bool tail;
     if (!at_work(p, head, t) || !at_find<BM>(p, t, start, len, tile, tail) || tail || tile * BM >= len) return;
@@ -507,6 +585,8 @@ __global__ __launch_bounds__(256, 2) void attn_delta_kernel(const mi_attn_args p
     const int32_t* const mask = p.key_mask ? p.key_mask + start : nullptr;
     u32x4 df[DP / 16], qf[DP / 16];                                    // qf: rows of out, or of q
     at_load_rows<DP>(df, p.dout, tok, head, p.hd, half);
+    float nl = p.lse[(int64_t)head * p.tokens + tok] * AT_LOG2E;
+    if (nl == -INFINITY) nl = INFINITY;                                // a row that attends nothing: p = 0
     float a = 0.0f, c = 0.0f;
     if (!BIAS && kend > (mask ? 512 : 128)) {
         at_load_rows<DP>(qf, p.out, tok, head, p.hd, half);
@@ -520,24 +600,15 @@ __global__ __launch_bounds__(256, 2) void attn_delta_kernel(const mi_attn_args p
         c = half == 0 ? 1.0f : 0.0f;
     } else {
         at_load_rows<DP>(qf, p.q, tok, head, p.hd, half);
-        AtStage<DP, 4> ks, vs;
-        ks.init(p.k, start, len, head / p.group, p.hd, wave, lane);
-        vs.init(p.v, start, len, head / p.group, p.hd, wave, lane);
-        const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds;
-        ks.issue(0, lds0, wave, mask);
-        vs.issue(0, lds0 + TB, wave, mask);
-        if constexpr (BIAS) at_fill_bias(p, head, vec);
-        float nl = p.lse[(int64_t)head * p.tokens + tok] * AT_LOG2E;
-        if (nl == -INFINITY) nl = INFINITY;                            // a row that attends nothing: p = 0
+        AtPipe<DP, NB> pipe;
+        pipe.a.init(p.k, start, 0, len, at_div(head, p.group_inv), p.hd, wave, lane);
+        pipe.b.init(p.v, start, 0, len, at_div(head, p.group_inv), p.hd, wave, lane);
+        pipe.start(lds, (kend + AT_KT - 1) / AT_KT, mask, wave);
+        if constexpr (BIAS) at_fill_bias(p, head, AT_LOG2E, vec);
         const int R = p.reach + AT_PAD;
-        for (int k0 = 0, buf = 0; k0 < kend; k0 += AT_KT, buf ^= 1) {
-            at_sync();
-            if (k0 + AT_KT < kend) {
-                ks.issue(k0 + AT_KT, lds0 + (buf ^ 1) * 2 * TB, wave, mask);
-                vs.issue(k0 + AT_KT, lds0 + (buf ^ 1) * 2 * TB + TB, wave, mask);
-            }
+        for (int k0 = 0; k0 < kend; k0 += AT_KT) {
+            const char* const Kt = lds + pipe.next(k0 / AT_KT);
             if (qw >= len || (p.causal && k0 > qw + 31)) continue;
-            const char* const Kt = lds + buf * 2 * TB;
             const uint64_t keys = at_keys(mask, k0, len, lane);
             const bool masked = ~keys != 0 || (p.causal && k0 + AT_KT - 1 > qw);
             const int rlo = k0 - (qw + 31), rhi = k0 + AT_KT - 1 - qw;
@@ -577,9 +648,13 @@ __global__ __launch_bounds__(256, 2) void attn_delta_kernel(const mi_attn_args p
     }
     a += at_other_half(a);
     c += at_other_half(c);
-    if (half == 0 && q < len) p.delta[(int64_t)head * p.tokens + tok] = c == 0.0f ? a : a / c;
+    if (half == 0 && q < len) {
+        p.delta[(int64_t)head * p.tokens + tok] = c == 0.0f ? a : a / c;
+        p.lse2[(int64_t)head * p.tokens + tok] = nl;
+    }
 }
 
+#define AT_DQ_BUFFERS(DP, BIAS) ((BIAS) ? ((DP) == 32 ? 3 : 2) : AT_BUFFERS(DP))
 // dQ: one block per (head, 128 query rows), like the forward pass: S^T = K Q^T and dP^T = V dO^T with the query on the lane,
 // dQ^T += K^T dS^T.
 //
@@ -591,9 +666,9 @@ template <int DP, bool F16, bool BIAS>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const mi_attn_args p)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    constexpr int BM = 128, TB = AtTile<DP>::BYTES;
+    constexpr int BM = 128, TB = AtTile<DP>::BYTES, NB = AT_DQ_BUFFERS(DP, BIAS);
     const int R = p.reach + AT_PAD, nvec = 2 * R + 1;
-    float* const skew0 = reinterpret_cast<float*>(lds + 4 * TB);       // BIAS: [4][32][64], the waves' images
+    float* const skew0 = reinterpret_cast<float*>(lds + NB * 2 * TB);       // BIAS: [4][32][64], the waves' images
     float* const vec = skew0 + 4 * 32 * 64;                            // the bias over r
     float* const dvec0 = vec + nvec;                                   // [4][nvec], the waves' sums over r
     int head, t, start, len, tile;
@@ -610,29 +685,26 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const mi_attn_args p)
     if (p.causal) tile = (len + BM - 1) / BM - 1 - tile;
     const int qw = tile * BM + wave * 32, q = qw + col;
     const int kend = p.causal ? (tile * BM + BM < len ? tile * BM + BM : len) : len;
-    const int kvh = head / p.group;
+    const int kvh = at_div(head, p.group_inv);
 
-    AtStage<DP, 4> ks, vs;
-    ks.init(p.k, start, len, kvh, p.hd, wave, lane);
-    vs.init(p.v, start, len, kvh, p.hd, wave, lane);
-    const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds;
     const int32_t* const mask = p.key_mask ? p.key_mask + start : nullptr;
-    ks.issue(0, lds0, wave, mask);
-    vs.issue(0, lds0 + TB, wave, mask);
+    AtPipe<DP, NB> pipe;
+    pipe.a.init(p.k, start, 0, len, kvh, p.hd, wave, lane);
+    pipe.b.init(p.v, start, 0, len, kvh, p.hd, wave, lane);
+    pipe.start(lds, (kend + AT_KT - 1) / AT_KT, mask, wave);
 
     u32x4 qf[DP / 16], df[DP / 16];
     const int64_t tok = start + (q < len ? q : len - 1);
     at_load_rows<DP>(qf, p.q, tok, head, p.hd, half);
     at_load_rows<DP>(df, p.dout, tok, head, p.hd, half);
     const float D = p.delta[(int64_t)head * p.tokens + tok];
-    float nl = p.lse[(int64_t)head * p.tokens + tok] * AT_LOG2E;
-    if (nl == -INFINITY || q >= len) nl = INFINITY;                    // a row that attends nothing, or is none: p = 0
+    const float nl = q < len ? p.lse2[(int64_t)head * p.tokens + tok] : INFINITY;   // +inf: p = 0
 
     float* const skew = skew0 + wave * 32 * 64;
     float* const dvec = dvec0 + wave * nvec;
     float farS[2] = {0.0f, 0.0f};                                      // sums of the tiles of one bucket, before and behind
     if constexpr (BIAS) {
-        at_fill_bias(p, head, vec);
+        at_fill_bias(p, head, p.scale_inv, vec);
 #pragma unroll
         for (int i = 0; i < 32; ++i) skew[i * 64 + lane] = 0.0f;
         for (int i = lane; i < nvec; i += 64) dvec[i] = 0.0f;
@@ -641,34 +713,24 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const mi_attn_args p)
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) dQ[dt] = at_zero16();
 
-    for (int k0 = 0, buf = 0; k0 < kend; k0 += AT_KT, buf ^= 1) {
-        at_sync();
-        if (k0 + AT_KT < kend) {
-            ks.issue(k0 + AT_KT, lds0 + (buf ^ 1) * 2 * TB, wave, mask);
-            vs.issue(k0 + AT_KT, lds0 + (buf ^ 1) * 2 * TB + TB, wave, mask);
-        }
+    for (int k0 = 0; k0 < kend; k0 += AT_KT) {
+        const char* const Kt = lds + pipe.next(k0 / AT_KT);
         if (qw >= len || (p.causal && k0 > qw + 31)) continue;
-        const char* const Kt = lds + buf * 2 * TB;
         const uint64_t keys = at_keys(mask, k0, len, lane);
         const bool masked = ~keys != 0 || (p.causal && k0 + AT_KT - 1 > qw);
         const int rlo = k0 - (qw + 31), rhi = k0 + AT_KT - 1 - qw;
         const bool near = BIAS && rhi > -p.reach && rlo < p.reach;
-        const float far = BIAS && !near ? vec[rhi <= -p.reach ? 0 : 2 * R] - nl : -nl;
+        const float far = BIAS && !near ? __builtin_fmaf(vec[rhi <= -p.reach ? 0 : 2 * R], p.scale_log2, -nl) : -nl;
         const float* const bv = vec + (k0 + 4 * half - q + R);
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
-            f32x16 S = at_zero16(), dP = at_zero16();
+            f32x16 S = at_first<F16>(near, bv + 32 * st, 1, at_rows<DP>(Kt, st, 0, col, half), qf[0]), dP = at_zero16();
 #pragma unroll
-            for (int s = 0; s < DP / 16; ++s) S = at_mfma<F16>(at_rows<DP>(Kt, st, s, col, half), qf[s], S);
+            for (int s = 1; s < DP / 16; ++s) S = at_mfma<F16>(at_rows<DP>(Kt, st, s, col, half), qf[s], S);
 #pragma unroll
             for (int s = 0; s < DP / 16; ++s) dP = at_mfma<F16>(at_rows<DP>(Kt + TB, st, s, col, half), df[s], dP);
-            if (near) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) S[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], p.scale_log2, bv[32 * st + 8 * (i >> 2) + (i & 3)] - nl));
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) S[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], p.scale_log2, far));
-            }
+            for (int i = 0; i < 16; ++i) S[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], p.scale_log2, far));
             // ds, over dp
 #pragma unroll
             for (int i = 0; i < 16; ++i) dP[i] = S[i] * (dP[i] - D);
@@ -742,14 +804,15 @@ template <int DP, bool F16, bool BIAS>
 __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(const mi_attn_args p)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    constexpr int BM = 128, TB = AtTile<DP>::BYTES;
-    float* const rowv = reinterpret_cast<float*>(lds + 4 * TB);        // [2][lse | D][64]
-    float* const vec = rowv + 256;
+    constexpr int BM = 128, TB = AtTile<DP>::BYTES, NB = AT_BUFFERS(DP), PER = 2 * AtStage<DP, 4>::NI + 1;
+    float* const rowv = reinterpret_cast<float*>(lds + NB * 2 * TB);   // [NB][lse in log2 units | D][64]
+    float* const vec = rowv + NB * 128;
     int kvh, t, start, len, tile;
     bool tail;
     if (!at_work(p, kvh, t) || !at_find<BM>(p, t, start, len, tile, tail)) return;
-    const int share = kvh % p.splits, heads = p.group / p.splits;      // (units are key heads x shares)
-    kvh /= p.splits;
+    const int unit = kvh, heads = p.share_heads;                       // (units are key heads x shares)
+    kvh = at_div(unit, p.splits_inv);
+    const int share = unit - kvh * p.splits;
     const int head0 = kvh * p.group + share * heads;
     if (tail) {
         if (share != 0) return;
@@ -772,55 +835,59 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(const 
     const int qfirst = p.causal ? tile * BM / AT_KT * AT_KT : 0;       // earlier queries attend no key of this block
     const int nq = (len - qfirst + AT_KT - 1) / AT_KT, n = nq * heads;
     AtStage<DP, 4> qs, ds;
-    float rowreg = 0.0f;
-    auto issue = [&](int it, int buf) __attribute__((always_inline)) {
-        const int head = head0 + it / nq, q0 = qfirst + it % nq * AT_KT;
-        qs.init(p.q, start, len, head, p.hd, wave, lane);
-        ds.init(p.dout, start, len, head, p.hd, wave, lane);
-        qs.issue(q0, lds0 + buf * 2 * TB, wave);
-        ds.issue(q0, lds0 + buf * 2 * TB + TB, wave);
-        if (wave < 2) {                                                // wave 0: log-sum-exp in log2 units, wave 1: D
-            const int q = q0 + lane;
-            const int64_t i = (int64_t)head * p.tokens + start + (q < len ? q : len - 1);
-            if (wave == 0) {
-                const float x = p.lse[i] * AT_LOG2E;
-                rowreg = q < len && x != -INFINITY ? x - AtPScale<F16>::log2 : INFINITY;
-            } else {
-                rowreg = q < len ? p.delta[i] * AtPScale<F16>::down : 0.0f;
-            }
+    int ihead = head0 - 1, iq = nq;                                    // the tile requested last: its head, its number
+    const float* rows = nullptr;
+    auto issue = [&](int slot) __attribute__((always_inline)) {
+        if (++iq >= nq) {
+            iq = 0;
+            ++ihead;
+            qs.init(p.q, start, qfirst, len, ihead, p.hd, wave, lane);
+            ds.init(p.dout, start, qfirst, len, ihead, p.hd, wave, lane);
+            rows = (wave & 1 ? p.delta : p.lse2) + (int64_t)ihead * p.tokens + start;
         }
+        qs.issue(lds0 + slot * 2 * TB, wave);
+        ds.issue(lds0 + slot * 2 * TB + TB, wave);
+        // 64 values of each row vector: even waves the log-sum-exp, odd ones D (waves 2 and 3 the same again)
+        const int q = qfirst + iq * AT_KT + lane;
+        at_dma4(rows + (q < len ? q : len - 1), lds0 + NB * 2 * TB + (unsigned)(slot * 128 + (wave & 1) * 64) * 4);
     };
     f32x16 dK[DP / 32], dV[DP / 32];
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) { dK[dt] = at_zero16(); dV[dt] = at_zero16(); }
-    issue(0, 0);
+#pragma unroll
+    for (int t2 = 0; t2 < NB - 1; ++t2) if (t2 < n) issue(t2);
     const int R = p.reach + AT_PAD;
     int bias_head = -1;
-    for (int it = 0, buf = 0; it < n; ++it, buf ^= 1) {
-        if (wave < 2) rowv[buf * 128 + wave * 64 + lane] = rowreg;
-        const int head = head0 + it / nq, q0 = qfirst + it % nq * AT_KT;
+    int head = head0, q0 = qfirst - AT_KT;
+    for (int it = 0, buf = NB - 1; it < n; ++it) {
+        q0 += AT_KT;
+        if (q0 >= len) {
+            q0 = qfirst;
+            ++head;
+        }
         if constexpr (BIAS) {
             if (head != bias_head) {
                 if (bias_head >= 0) at_sync();                         // the last head's vector has been read
-                at_fill_bias(p, head, vec);
+                at_fill_bias(p, head, p.scale_inv, vec);
                 bias_head = head;
             }
         }
-        at_sync();
-        if (it + 1 < n) issue(it + 1, buf ^ 1);
+        at_arrive<PER>(n - 1 - it < NB - 2 ? n - 1 - it : NB - 2);
+        if (it + NB - 1 < n) issue(buf);
+        buf = buf + 1 == NB ? 0 : buf + 1;
         if (kw >= len || (p.causal && q0 + AT_KT - 1 < kw)) continue;
         const char* const Qt = lds + buf * 2 * TB;
         const char* const Dt = Qt + TB;
-        const bool diag = p.causal && q0 < kw + 31;
+        const bool edge = (p.causal && q0 < kw + 31) || q0 + AT_KT > len;   // rows that do not attend, or are none
         const int rlo = kw - (q0 + AT_KT - 1), rhi = kw + 31 - q0;
         const bool near = BIAS && rhi > -p.reach && rlo < p.reach;
-        const float far = BIAS && !near ? vec[rhi <= -p.reach ? 0 : 2 * R] : 0.0f;
+        const float add = AtPScale<F16>::log2 + (BIAS && !near ? vec[rhi <= -p.reach ? 0 : 2 * R] * p.scale_log2 : 0.0f);
         const int at = key - q0 - 4 * half + R;
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
-            f32x16 S = at_zero16(), dP = at_zero16();
+            f32x16 S = at_first<F16>(near, vec + at - 32 * st, -1, at_rows<DP>(Qt, st, 0, col, half), kf[0]), dP = at_zero16();
 #pragma unroll
-            for (int s = 0; s < DP / 16; ++s) S = at_mfma<F16>(at_rows<DP>(Qt, st, s, col, half), kf[s], S);
+            for (int s = 1; s < DP / 16; ++s) S = at_mfma<F16>(at_rows<DP>(Qt, st, s, col, half), kf[s], S);
 #pragma unroll
             for (int s = 0; s < DP / 16; ++s) dP = at_mfma<F16>(at_rows<DP>(Dt, st, s, col, half), vf[s], dP);
 #pragma unroll
@@ -831,15 +898,16 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(const 
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int i = 4 * g + e;
-                    const float b = near ? vec[at - 32 * st - 8 * g - e] : far;
-                    S[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], p.scale_log2, b - nls[e]));
-                    dP[i] = S[i] * __builtin_fmaf(dP[i], AtPScale<F16>::down, -Drs[e]);
+                    S[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], p.scale_log2, add - nls[e]));
+                    dP[i] = S[i] * ((dP[i] - Drs[e]) * AtPScale<F16>::down);
                 }
             }
-            if (diag) {
+            if (edge) {
+                const int first = p.causal ? key - q0 - 32 * st - 4 * half : -AT_KT, end = len - q0 - 32 * st - 4 * half;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const bool ok = q0 + 32 * st + 8 * (i >> 2) + 4 * half + (i & 3) >= key;
+                    const int r = 8 * (i >> 2) + (i & 3);
+                    const bool ok = r >= first && r < end;
                     S[i] = ok ? S[i] : 0.0f;
                     dP[i] = ok ? dP[i] : 0.0f;
                 }
@@ -917,17 +985,17 @@ __global__ __launch_bounds__(1024) void attn_dtable_kernel(const mi_attn_args p)
 static int gcd_int(int a, int b) { while (b) { const int t = a % b; a = b; b = t; } return a; }
 
 // The grid over `heads` heads and tiles of BM rows (see at_work).
-static unsigned at_schedule(mi_attn_args* a, int heads, int BM)
+static dim3 at_schedule(mi_attn_args* a, int heads, int BM)
 {
     const int64_t tiles = a->offsets ? a->tokens / BM + a->nseq + (a->zero_tail ? 1 : 0)
                                      : (int64_t)a->nseq * ((a->uniform_len + BM - 1) / BM);
     const int g = gcd_int(heads, 8);
     a->tiles = (int)tiles;
-    a->parts = 8 / g;
-    a->units_per_xcd = heads * a->parts / 8;
-    a->tiles_per_unit = (int)((tiles + a->parts - 1) / a->parts);
-    return (unsigned)((int64_t)heads * a->parts * a->tiles_per_unit);
+    a->parts_log2 = g == 8 ? 0 : g == 4 ? 1 : g == 2 ? 2 : 3;
+    a->units_per_xcd = heads / g;
+    return dim3((unsigned)(8 * ((tiles + 8 / g - 1) >> a->parts_log2)), (unsigned)a->units_per_xcd);
 }
+static uint32_t inv32(int d) { return d <= 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + d - 1) / d); }
 
 // Leave for more than the default 64 KB of dynamic LDS, asked for once per kernel and device.
 template <auto KERNEL>
@@ -944,22 +1012,26 @@ static int at_lds(size_t bytes)
     return MI_OK;
 }
 
+template <int DP, bool F16, bool BIAS, int KS>
+static int launch_fwd(hipStream_t st, mi_attn_args& a)
+{
+    const dim3 grid = at_schedule(&a, a.heads, 128 / KS);
+    if (grid.x == 0) return MI_OK;
+    size_t smem = AT_BUFFERS(DP) * 2 * AtTile<DP>::BYTES + (BIAS ? (2 * (size_t)(a.reach + AT_PAD) + 1) * 4 : 0);
+    if (KS == 2 && smem < (size_t)2 * (DP / 2 + 3) * 64 * 4) smem = (size_t)2 * (DP / 2 + 3) * 64 * 4;
+    MI_TRY((at_lds<&attn_fwd_kernel<DP, F16, BIAS, KS>>(smem)));
+    attn_fwd_kernel<DP, F16, BIAS, KS><<<grid, 256, smem, st>>>(a);
+    MI_HIP(hipGetLastError());
+    return MI_OK;
+}
+
 template <int DP, bool F16>
 static int launch_fwd(hipStream_t st, mi_attn_args& a)
 {
-    const unsigned grid = at_schedule(&a, a.heads, 128);
-    size_t smem = 4 * AtTile<DP>::BYTES;
-    if (grid == 0) return MI_OK;
-    if (a.table) {
-        smem += (2 * (size_t)(a.reach + AT_PAD) + 1) * sizeof(float);
-        MI_TRY((at_lds<&attn_fwd_kernel<DP, F16, true, 1>>(smem)));
-        attn_fwd_kernel<DP, F16, true, 1><<<grid, 256, smem, st>>>(a);
-    } else {
-        MI_TRY((at_lds<&attn_fwd_kernel<DP, F16, false, 1>>(smem)));
-        attn_fwd_kernel<DP, F16, false, 1><<<grid, 256, smem, st>>>(a);
-    }
-    MI_HIP(hipGetLastError());
-    return MI_OK;
+    static const int force = getenv("AT_KS") ? atoi(getenv("AT_KS")) : 0;
+    const bool split = force ? force == 2 : false;
+    if (a.table) return split ? launch_fwd<DP, F16, true, 2>(st, a) : launch_fwd<DP, F16, true, 1>(st, a);
+    return split ? launch_fwd<DP, F16, false, 2>(st, a) : launch_fwd<DP, F16, false, 1>(st, a);
 }
 
 int mi_launch_attention(hipStream_t st, mi_attn_args a, int dtype)
@@ -984,7 +1056,7 @@ static int at_dkv_splits(const mi_attn_args& a)
 
 size_t mi_attn_backward_bytes(const mi_attn_args& a)
 {
-    const size_t delta = mi_round_up((int64_t)a.heads * a.tokens * 4, 256);
+    const size_t delta = mi_round_up((int64_t)a.heads * a.tokens * 8, 256);
     const int splits = at_dkv_splits(a);
     const size_t join = splits > 1 ? (size_t)mi_round_up((int64_t)splits * 2 * a.tokens * (a.heads / a.group) * a.hd * 4, 256) : 0;
     const int64_t tiles = a.offsets ? a.tokens / 128 + a.nseq + 1 : (int64_t)a.nseq * ((a.uniform_len + 127) / 128);
@@ -994,9 +1066,9 @@ size_t mi_attn_backward_bytes(const mi_attn_args& a)
 template <int DP, bool F16, bool BIAS>
 static int launch_dq(hipStream_t st, mi_attn_args& a)
 {
-    const unsigned grid = at_schedule(&a, a.heads, 128);
-    if (grid == 0) return MI_OK;
-    const size_t smem = 4 * AtTile<DP>::BYTES + (BIAS ? (4 * 32 * 64 + 5 * (2 * (size_t)(a.reach + AT_PAD) + 1)) * 4 : 0);
+    const dim3 grid = at_schedule(&a, a.heads, 128);
+    if (grid.x == 0) return MI_OK;
+    const size_t smem = AT_DQ_BUFFERS(DP, BIAS) * 2 * AtTile<DP>::BYTES + (BIAS ? (4 * 32 * 64 + 5 * (2 * (size_t)(a.reach + AT_PAD) + 1)) * 4 : 0);
     MI_TRY((at_lds<&attn_dq_kernel<DP, F16, BIAS>>(smem)));
     attn_dq_kernel<DP, F16, BIAS><<<grid, 256, smem, st>>>(a);
     MI_HIP(hipGetLastError());
@@ -1006,9 +1078,9 @@ static int launch_dq(hipStream_t st, mi_attn_args& a)
 template <int DP, bool F16, bool BIAS>
 static int launch_delta(hipStream_t st, mi_attn_args& a)
 {
-    const unsigned grid = at_schedule(&a, a.heads, 128);
-    if (grid == 0) return MI_OK;
-    const size_t smem = 4 * AtTile<DP>::BYTES + (BIAS ? (size_t)(2 * (a.reach + AT_PAD) + 1) * 4 : 0);
+    const dim3 grid = at_schedule(&a, a.heads, 128);
+    if (grid.x == 0) return MI_OK;
+    const size_t smem = AT_BUFFERS(DP) * 2 * AtTile<DP>::BYTES + (BIAS ? (size_t)(2 * (a.reach + AT_PAD) + 1) * 4 : 0);
     MI_TRY((at_lds<&attn_delta_kernel<DP, F16, BIAS>>(smem)));
     attn_delta_kernel<DP, F16, BIAS><<<grid, 256, smem, st>>>(a);
     MI_HIP(hipGetLastError());
@@ -1026,9 +1098,9 @@ static int launch_bwd(hipStream_t st, mi_attn_args& a)
         attn_dtable_kernel<<<(unsigned)a.heads, 1024, 0, st>>>(a);
         MI_HIP(hipGetLastError());
     }
-    const unsigned grid = at_schedule(&a, a.heads / a.group * a.splits, 128);
-    if (grid == 0) return MI_OK;
-    const size_t smem = 4 * AtTile<DP>::BYTES + 1024 + (a.table ? (size_t)(2 * (a.reach + AT_PAD) + 1) * 4 : 0);
+    const dim3 grid = at_schedule(&a, a.heads / a.group * a.splits, 128);
+    if (grid.x == 0) return MI_OK;
+    const size_t smem = AT_BUFFERS(DP) * (2 * AtTile<DP>::BYTES + 512) + (a.table ? (size_t)(2 * (a.reach + AT_PAD) + 1) * 4 : 0);
     if (a.table) {
         MI_TRY((at_lds<&attn_dkv_kernel<DP, F16, true>>(smem)));
         attn_dkv_kernel<DP, F16, true><<<grid, 256, smem, st>>>(a);
@@ -1047,8 +1119,11 @@ static int launch_bwd(hipStream_t st, mi_attn_args& a)
 int mi_launch_attention_backward(hipStream_t st, mi_attn_args a, int dtype, void* workspace)
 {
     a.delta = (float*)workspace;
+    a.lse2 = a.delta + (int64_t)a.heads * a.tokens;
     a.splits = at_dkv_splits(a);
-    a.parts_kv = (float*)((char*)workspace + mi_round_up((int64_t)a.heads * a.tokens * 4, 256));
+    a.splits_inv = inv32(a.splits);
+    a.share_heads = a.group / a.splits;
+    a.parts_kv = (float*)((char*)workspace + mi_round_up((int64_t)a.heads * a.tokens * 8, 256));
     a.partial = (float*)((char*)a.parts_kv + (a.splits > 1 ? mi_round_up((int64_t)a.splits * 2 * a.tokens * (a.heads / a.group) * a.hd * 4, 256) : 0));
     const bool f16 = dtype == MI_DTYPE_F16;
     if (a.hd <= 32) return f16 ? launch_bwd<32, true>(st, a) : launch_bwd<32, false>(st, a);
@@ -1072,6 +1147,7 @@ int mi_attn_buckets(const char* who, mi_attn_args* a, int buckets, int max_dista
     // border t: the least whole d with d^(n - m) >= max_distance^t m^(n - m - t).  Found in floating point; a real border within
     // 1e-12 of a whole number (far below the distance of any other border from one, for these sizes) is that number.
     int reach = m;
+    for (int32_t& x : a->border) x = INT32_MAX;
     for (int t = 1; t <= a->nborder; ++t) {
         const double x = m * exp((double)t / (n - m) * log((double)max_distance / m));
         int d = (int)ceil(x * (1.0 - 1e-12));
@@ -1107,7 +1183,7 @@ static int fill_args(const char* who, mi_ctx* ctx, const mi_attention_config* c,
     MI_REQUIRE(c->dtype == MI_DTYPE_BF16 || c->dtype == MI_DTYPE_F16, "%s: dtype %d is not MI_DTYPE_BF16 or MI_DTYPE_F16", who, c->dtype);
     MI_REQUIRE(c->heads > 0 && c->heads <= 65535 && c->kv_heads > 0 && c->heads % c->kv_heads == 0, "%s: heads %d must be a positive multiple of kv_heads %d", who, c->heads, c->kv_heads);
     MI_REQUIRE(c->head_dim > 0 && c->head_dim % 8 == 0 && c->head_dim <= 128, "%s: head_dim %d must be a multiple of 8 up to 128", who, c->head_dim);
-    MI_REQUIRE(c->scale > 0.0f && c->scale <= FLT_MAX / 2, "%s: scale must be positive and finite", who);
+    MI_REQUIRE(c->scale >= 1e-20f && c->scale <= 1e20f, "%s: scale must be between 1e-20 and 1e20", who);
     MI_REQUIRE(tokens >= 0 && tokens < ((int64_t)1 << 31) - 4096, "%s: %lld tokens out of range", who, (long long)tokens);
     MI_REQUIRE(nseq >= 0 && nseq < ((int64_t)1 << 24), "%s: %lld sequences out of range", who, (long long)nseq);
     MI_REQUIRE(offsets || (nseq == 0 ? tokens == 0 : tokens % nseq == 0), "%s: %lld tokens are not %lld sequences of one length", who, (long long)tokens, (long long)nseq);
@@ -1128,13 +1204,15 @@ static int fill_args(const char* who, mi_ctx* ctx, const mi_attention_config* c,
     a->uniform_len = offsets || nseq == 0 ? 0 : (int)(tokens / nseq);
     a->heads = c->heads;
     a->group = c->heads / c->kv_heads;
+    a->group_inv = inv32(a->group);
     a->hd = c->head_dim;
     a->causal = c->causal != 0;
     a->zero_tail = c->zero_tail != 0;
     a->scale = c->scale;
     a->scale_log2 = c->scale * AT_LOG2E;
-    // one launch: heads x tiles of at least 64 rows, below 2^31 blocks
-    MI_REQUIRE((tokens / 64 + nseq + 9) * (int64_t)c->heads < ((int64_t)1 << 31) - 1, "%s: %lld tokens x %d heads are too many for one call", who, (long long)tokens, c->heads);
+    a->scale_inv = 1.0f / c->scale;
+    // one launch: tiles of at least 64 rows on x, heads on y, below 2^32 threads and 2^31 blocks
+    MI_REQUIRE((tokens / 64 + nseq + 9) * 8 * 256 < ((int64_t)1 << 32) - 1 && (tokens / 64 + nseq + 9) * (int64_t)c->heads < ((int64_t)1 << 31) - 1, "%s: %lld tokens x %d heads are too many for one call", who, (long long)tokens, c->heads);
     return MI_OK;
 }
 

@@ -81,6 +81,7 @@ BAD = [
     (dict(change=dict(head_dim=136)), "head_dim"),
     (dict(change=dict(scale=0.0)), "scale"),
     (dict(change=dict(scale=-1.0)), "scale"),
+    (dict(change=dict(scale=1e-30)), "scale"),
     (dict(change=dict(scale=float("nan"))), "scale"),
     (dict(change=dict(scale=float("inf"))), "scale"),
     (dict(tokens=-1), "tokens"),
