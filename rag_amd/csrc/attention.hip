@@ -10,6 +10,7 @@
 #include <math.h>
 #include <stdlib.h>
 #include <atomic>
+#include <type_traits>
 #include "attention.h"
 #include "kernels.h"
 
@@ -26,6 +27,7 @@ typedef __attribute__((address_space(3))) tr4_t tr4_lds_t;
 #define AT_LN2 0.6931471805599453f
 #define AT_KT 64                       // rows of the staged operand per tile
 
+template <int V> using at_int = std::integral_constant<int, V>;
 template <bool F16> __device__ __forceinline__ f32x16 at_mfma(u32x4 a, u32x4 b, f32x16 c)
 {
     if constexpr (F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -357,28 +359,35 @@ __device__ __forceinline__ float at_bias(const mi_attn_args& p, int head, int r,
     const float x = p.table[(int64_t)at_bucket(p, r) * p.heads + head];
     return (fabsf(x) <= FLT_MAX ? fminf(fmaxf(x, -AT_BIAS_MOST), AT_BIAS_MOST) : x) * unit;
 }
-__device__ __forceinline__ void at_fill_bias(const mi_attn_args& p, int head, float unit, float* vec)
+__device__ __forceinline__ void at_fill_bias(const mi_attn_args& p, int head, float unit, float shift, float* vec)
 {
     const int R = p.reach + AT_PAD;
-    for (int i = threadIdx.x; i < 2 * R + 1; i += blockDim.x) vec[i] = at_bias(p, head, i - R, unit);
+    for (int i = threadIdx.x; i < 2 * R + 1; i += blockDim.x) vec[i] = at_bias(p, head, i - R, unit) + shift;
 }
 
-// Which of the 64 keys at k0 are keys of the sequence that the mask leaves (bit = key - k0); the wave's lanes ask for one each.
+// Which of the 64 keys at k0 the mask leaves (bit = key - k0); the wave's lanes ask for one each.
 __device__ __forceinline__ uint64_t at_keys(const int32_t* mask, int k0, int len, int lane)
 {
-    if (!mask && k0 + AT_KT <= len) return ~0ull;
     const int key = k0 + lane;
-    return __builtin_amdgcn_ballot_w64(key < len && (!mask || mask[key < len ? key : len - 1] != 0));
+    return __builtin_amdgcn_ballot_w64(key < len && mask[key < len ? key : len - 1] != 0);
 }
-// ... and of the 32 of block st those that this lane's query attends, bit 8 g + i for its register 4 g + i; ahead = query - k0
-__device__ __forceinline__ uint32_t at_allowed(const mi_attn_args& p, uint64_t keys, int st, int ahead, int half)
+// Calls f(i, attended) for the registers of a block of scores, 32 keys from k on, one query a lane (register 4 g + i is key
+// k + 8 g + 4 half + i), where not all are attended; keys: the block's bits of at_keys, used where there is a mask.
+template <class F>
+__device__ __forceinline__ void at_unattended(const mi_attn_args& p, const int32_t* mask, uint32_t keys, int k, int qw, int q, int len, int half, F&& f)
 {
-    uint32_t ok = (uint32_t)(keys >> (32 * st));
-    if (p.causal) {
-        const int lim = ahead - 32 * st;                               // the last attended key of the block
-        ok = lim >= 31 ? ok : lim < 0 ? 0u : ok & ((2u << lim) - 1u);
+    if (k + 32 <= len && !(p.causal && k + 31 > qw) && !(mask && keys != 0xFFFFFFFFu)) return;
+    int lim = len - 1 - k;                                             // the last attended key but for the mask
+    if (p.causal && q - k < lim) lim = q - k;
+    lim -= 4 * half;
+    if (mask) {
+        uint32_t ok = keys >> (4 * half);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) f(i, 8 * (i >> 2) + (i & 3) <= lim && ((ok >> (8 * (i >> 2) + (i & 3))) & 1u));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) f(i, 8 * (i >> 2) + (i & 3) <= lim);
     }
-    return ok >> (4 * half);
 }
 
 // The first of a score block's products, on the bias where it is not one value for the tile: 8 g + i steps on from bv
@@ -397,8 +406,7 @@ __device__ __forceinline__ f32x16 at_first(bool near, const float* bv, int step,
 // ---------------------------------------------------------------- forward
 #define AT_BUFFERS(DP) ((DP) == 32 ? 4 : (DP) == 64 ? 3 : 2)          // what leaves LDS for as many blocks as the registers do
 // One block per (head, 128 / KS query rows): four waves, each 32 queries by every KS-th 32-key block of the K and V tiles, which come by
-// LDS-DMA, 64 keys at a time, one barrier per tile.  The running maximum is an exponent reference that only has to keep exp2 in
-// range: it moves, and O and l are rescaled, when a tile's maximum exceeds it by more than 2^8 (fp16: 2^15).  With KS = 2 the two
+// LDS-DMA, 64 keys at a time, one barrier per tile.  With KS = 2 the two
 // waves of a query join their sums through LDS at the end: half the time per tile and twice the blocks, for calls of few blocks.
 template <int DP, bool F16, bool BIAS, int KS>
 __global__ __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) void attn_fwd_kernel(const mi_attn_args p)
@@ -430,58 +438,49 @@ __global__ __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) void attn_fwd
     pipe.a.init(p.k, start, 0, len, kvh, p.hd, wave, lane);
     pipe.b.init(p.v, start, 0, len, kvh, p.hd, wave, lane);
     pipe.start(lds, (kend + AT_KT - 1) / AT_KT, mask, wave);
-    if constexpr (BIAS) at_fill_bias(p, head, AT_LOG2E, vec);
+    if constexpr (BIAS) at_fill_bias(p, head, AT_LOG2E, F16 ? 8.0f : 0.0f, vec);
 
     f32x16 O[DP / 32];
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) O[dt] = at_zero16();
     // the reference starts at a usual place and stays while the first tile's maximum lies within 2^8 of it; bf16 has fp32's range,
     // fp16 takes it 2^8 lower so that the sum is at least 1, and p up to 2^15
-    constexpr float M0 = F16 ? -8.0f : 0.0f, HIGH = F16 ? 15.0f : 8.0f, LOW = F16 ? 0.0f : -8.0f;
-    float m = M0, low = LOW, l = 0.0f;                                 // low = -inf once a finite score has been seen
+    constexpr float REF0 = F16 ? -8.0f : 0.0f, HIGH = F16 ? 15.0f : 8.0f, LOW = F16 ? 0.0f : -8.0f;
+    float m = 0.0f, low = LOW, l = 0.0f;                               // reference = REF0 + m; low = -inf once a finite score has been seen
+    bool moved = false;                                                // some lane's m is not 0
     const int R = p.reach + AT_PAD;
     const float c = p.scale_log2;
-    for (int k0 = 0; k0 < kend; k0 += AT_KT) {
-        const char* const Kt = lds + pipe.next(k0 / AT_KT);
-        const char* const Vt = Kt + TB;
-        // nothing for this wave (it has met the barrier)
+    // One tile, in the forms that the loops below need: with and without unattended keys, with the bias one value (FAR) or many,
+    // from which m is taken or, while it is 0 on every lane, not.  Each is a straight run of code in a loop of its own: where
+    // forms meet in one loop hipcc copies O for each.
+    constexpr int FAR = 0, NEAR0 = 1, NEARM = 2;
+    auto compute = [&](auto masked_, auto form_, int k0, const char* Kt) __attribute__((always_inline)) {
+        constexpr bool MASKED = decltype(masked_)::value;
+        constexpr int FORM = decltype(form_)::value;
         const int kw = k0 + 32 * s0;
-        if (qw >= len || kw >= kend || (p.causal && kw > qw + 31)) continue;
-        const uint64_t keys = at_keys(mask, k0, len, lane);
-        const bool masked = ~keys != 0 || (p.causal && kw + 32 * NS - 1 > qw);
-
+        const uint64_t keys = MASKED && mask ? at_keys(mask, k0, len, lane) : 0;
+        const float less = BIAS ? vec[kw < qw ? 0 : 2 * R] - m : -REF0 - m;
         f32x16 S[NS];
-        float less = -m;                                               // what is left to add to c S
-        bool near = false;
-        const float* bv = vec;
-        if constexpr (BIAS) {
-            const int rlo = kw - (qw + 31), rhi = kw + 32 * NS - 1 - qw;
-            near = rhi > -p.reach && rlo < p.reach;
-            bv = vec + (kw + 4 * half - q + R);
-            if (!near) less += vec[rhi <= -p.reach ? 0 : 2 * R];
-        }
 #pragma unroll
         for (int n = 0; n < NS; ++n)
 #pragma unroll
             for (int s = 0; s < DP / 16; ++s) S[n] = at_mfma<F16>(at_rows<DP>(Kt, s0 + n, s, col, half), qf[s], s == 0 ? at_zero16() : S[n]);
-        // score in log2 units, less the reference
-        if (near) {
+        const float* const bv = vec + (kw + 4 * half - q + R);         // (less the reference's start)
 #pragma unroll
-            for (int n = 0; n < NS; ++n)
+        for (int n = 0; n < NS; ++n) {
+            int lim = 0;                                               // the last attended key but for the mask
+            uint32_t ok = 0;
+            if constexpr (MASKED) {
+                lim = len - 1 - kw - 32 * n;
+                if (p.causal && q - kw - 32 * n < lim) lim = q - kw - 32 * n;
+                lim -= 4 * half;
+                ok = (uint32_t)(keys >> (32 * (s0 + n))) >> (4 * half);
+            }
 #pragma unroll
-                for (int i = 0; i < 16; ++i) S[n][i] = __builtin_fmaf(S[n][i], c, bv[32 * n + 8 * (i >> 2) + (i & 3)] - m);
-        } else {
-#pragma unroll
-            for (int n = 0; n < NS; ++n)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) S[n][i] = __builtin_fmaf(S[n][i], c, less);
-        }
-        if (masked) {
-#pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                const uint32_t ok = at_allowed(p, keys, s0 + n, q - k0, half);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) S[n][i] = (ok >> (8 * (i >> 2) + (i & 3))) & 1u ? S[n][i] : -INFINITY;
+            for (int i = 0; i < 16; ++i) {
+                const int r = 8 * (i >> 2) + (i & 3);
+                S[n][i] = __builtin_fmaf(S[n][i], c, FORM == FAR ? less : FORM == NEARM ? bv[32 * n + r] - m : bv[32 * n + r]);
+                if constexpr (MASKED) S[n][i] = r <= lim && (!mask || ((ok >> r) & 1u)) ? S[n][i] : -INFINITY;
             }
         }
         float top = S[0][0];
@@ -497,6 +496,7 @@ __global__ __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) void attn_fwd
             const float up = move ? top : 0.0f;
             const float alpha = low > -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(-up);   // (nothing summed before the first)
             m += up;
+            moved = true;
             l *= alpha;
 #pragma unroll
             for (int dt = 0; dt < DP / 32; ++dt) O[dt] = O[dt] * alpha;
@@ -519,9 +519,42 @@ __global__ __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) void attn_fwd
 #pragma unroll
             for (int i = 0; i < 4; ++i) pf[i] = at_pack2<F16>(S[kk >> 1][8 * (kk & 1) + 2 * i], S[kk >> 1][8 * (kk & 1) + 2 * i + 1]);
 #pragma unroll
-            for (int dt = 0; dt < DP / 32; ++dt) O[dt] = at_mfma<F16>(at_cols<DP>(Vt, 2 * s0 + kk, dt, lane), pf, O[dt]);
+            for (int dt = 0; dt < DP / 32; ++dt) O[dt] = at_mfma<F16>(at_cols<DP>(Kt + TB, 2 * s0 + kk, dt, lane), pf, O[dt]);
+        }
+    };
+    // tiles: [0, far0) all before the bias's reach, [far0, far1) within it, [far1, plain) behind it, [plain, live) with unattended
+    // keys, [live, all) nothing for this wave but the barriers
+    const int all = pipe.n, lim = p.causal && qw + 1 < len ? qw + 1 : len;
+    int live = 0, plain = 0, far0 = 0, far1 = 0;
+    if (qw < len) {
+        const int end = p.causal && qw + 32 < kend ? qw + 32 : kend;
+        live = end <= 32 * s0 ? 0 : (end - 32 * s0 + AT_KT - 1) / AT_KT;
+        plain = mask || lim < 32 * (NS + s0) ? 0 : (lim - 32 * (NS + s0)) / AT_KT + 1;
+        if (plain > live) plain = live;
+        if constexpr (BIAS) {
+            const int x = qw - p.reach - 32 * (NS + s0) + 1, y = qw + 31 + p.reach - 32 * s0;   // before: k0 <= x; behind: k0 >= y
+            far0 = x < 0 ? 0 : x / AT_KT + 1;
+            far1 = (y + AT_KT - 1) / AT_KT;
         }
     }
+    const int end0 = BIAS ? (far0 < plain ? far0 : plain) : plain, end1 = far1 < plain ? far1 : plain;
+    auto run = [&](auto masked_, auto form_, int t) __attribute__((always_inline)) { compute(masked_, form_, t * AT_KT, lds + pipe.next(t)); };
+    using std::false_type;
+    using std::true_type;
+    int t2 = 0;
+    for (; t2 < end0; ++t2) run(false_type{}, at_int<FAR>{}, t2);
+    if constexpr (BIAS) {
+        for (; t2 < end1 && !moved; ++t2) run(false_type{}, at_int<NEAR0>{}, t2);
+        for (; t2 < end1; ++t2) run(false_type{}, at_int<NEARM>{}, t2);
+        for (; t2 < plain; ++t2) run(false_type{}, at_int<FAR>{}, t2);
+        for (; t2 < live; ++t2) {
+            if (t2 < far0 || t2 >= far1) run(true_type{}, at_int<FAR>{}, t2);
+            else run(true_type{}, at_int<NEARM>{}, t2);
+        }
+    } else {
+        for (; t2 < live; ++t2) run(true_type{}, at_int<FAR>{}, t2);
+    }
+    for (; t2 < all; ++t2) (void)pipe.next(t2);
     float sum = l + at_other_half(l);
     if constexpr (KS == 2) {
         // waves 2 and 3 hand over reference, sum and O; rows of 64 lanes, one register each
@@ -553,7 +586,7 @@ __global__ __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) void attn_fwd
     if (q < len) {
         at_store_row<DP, F16>(p.out, start + q, head, p.hd, half, O, sum == 0.0f ? 0.0f : 1.0f / sum);
         if (p.lse && half == 0)
-            p.lse[(int64_t)head * p.tokens + start + q] = sum == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * AT_LN2;
+            p.lse[(int64_t)head * p.tokens + start + q] = sum == 0.0f ? -INFINITY : (REF0 + m + __builtin_amdgcn_logf(sum)) * AT_LN2;
     }
 }
 
@@ -604,19 +637,19 @@ __global__ __launch_bounds__(256, 2) void attn_delta_kernel(const mi_attn_args p
         pipe.a.init(p.k, start, 0, len, at_div(head, p.group_inv), p.hd, wave, lane);
         pipe.b.init(p.v, start, 0, len, at_div(head, p.group_inv), p.hd, wave, lane);
         pipe.start(lds, (kend + AT_KT - 1) / AT_KT, mask, wave);
-        if constexpr (BIAS) at_fill_bias(p, head, AT_LOG2E, vec);
+        if constexpr (BIAS) at_fill_bias(p, head, AT_LOG2E, 0.0f, vec);
         const int R = p.reach + AT_PAD;
         for (int k0 = 0; k0 < kend; k0 += AT_KT) {
             const char* const Kt = lds + pipe.next(k0 / AT_KT);
             if (qw >= len || (p.causal && k0 > qw + 31)) continue;
-            const uint64_t keys = at_keys(mask, k0, len, lane);
-            const bool masked = ~keys != 0 || (p.causal && k0 + AT_KT - 1 > qw);
+            const uint64_t keys = mask ? at_keys(mask, k0, len, lane) : 0;
             const int rlo = k0 - (qw + 31), rhi = k0 + AT_KT - 1 - qw;
             const bool near = BIAS && rhi > -p.reach && rlo < p.reach;
             const float far = BIAS && !near ? vec[rhi <= -p.reach ? 0 : 2 * R] - nl : -nl;
             const float* const bv = vec + (k0 + 4 * half - q + R);
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
+                if (st > 0 && (k0 + 32 >= kend || (p.causal && k0 + 32 > qw + 31))) break;
                 f32x16 S = at_zero16(), dP = at_zero16();
 #pragma unroll
                 for (int s = 0; s < DP / 16; ++s) S = at_mfma<F16>(at_rows<DP>(Kt, st, s, col, half), qf[s], S);
@@ -629,15 +662,10 @@ __global__ __launch_bounds__(256, 2) void attn_delta_kernel(const mi_attn_args p
 #pragma unroll
                     for (int i = 0; i < 16; ++i) S[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], p.scale_log2, far));
                 }
-                if (masked) {
-                    const uint32_t ok = at_allowed(p, keys, st, q - k0, half);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const bool on = (ok >> (8 * (i >> 2) + (i & 3))) & 1u;
-                        S[i] = on ? S[i] : 0.0f;
-                        dP[i] = on ? dP[i] : 0.0f;
-                    }
-                }
+                at_unattended(p, mask, (uint32_t)(keys >> (32 * st)), k0 + 32 * st, qw, q, len, half, [&](int i, bool on) __attribute__((always_inline)) {
+                    S[i] = on ? S[i] : 0.0f;
+                    dP[i] = on ? dP[i] : 0.0f;
+                });
                 float a1 = 0.0f, c1 = 0.0f;                            // (short chains: a long row's sums stay exact to fp32's last bits)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) { a1 = __builtin_fmaf(S[i], dP[i], a1); c1 += S[i]; }
@@ -704,7 +732,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const mi_attn_args p)
     float* const dvec = dvec0 + wave * nvec;
     float farS[2] = {0.0f, 0.0f};                                      // sums of the tiles of one bucket, before and behind
     if constexpr (BIAS) {
-        at_fill_bias(p, head, p.scale_inv, vec);
+        at_fill_bias(p, head, p.scale_inv, 0.0f, vec);
 #pragma unroll
         for (int i = 0; i < 32; ++i) skew[i * 64 + lane] = 0.0f;
         for (int i = lane; i < nvec; i += 64) dvec[i] = 0.0f;
@@ -716,14 +744,14 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const mi_attn_args p)
     for (int k0 = 0; k0 < kend; k0 += AT_KT) {
         const char* const Kt = lds + pipe.next(k0 / AT_KT);
         if (qw >= len || (p.causal && k0 > qw + 31)) continue;
-        const uint64_t keys = at_keys(mask, k0, len, lane);
-        const bool masked = ~keys != 0 || (p.causal && k0 + AT_KT - 1 > qw);
+        const uint64_t keys = mask ? at_keys(mask, k0, len, lane) : 0;
         const int rlo = k0 - (qw + 31), rhi = k0 + AT_KT - 1 - qw;
         const bool near = BIAS && rhi > -p.reach && rlo < p.reach;
         const float far = BIAS && !near ? __builtin_fmaf(vec[rhi <= -p.reach ? 0 : 2 * R], p.scale_log2, -nl) : -nl;
         const float* const bv = vec + (k0 + 4 * half - q + R);
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
+            if (st > 0 && (k0 + 32 >= kend || (p.causal && k0 + 32 > qw + 31))) break;
             f32x16 S = at_first<F16>(near, bv + 32 * st, 1, at_rows<DP>(Kt, st, 0, col, half), qf[0]), dP = at_zero16();
 #pragma unroll
             for (int s = 1; s < DP / 16; ++s) S = at_mfma<F16>(at_rows<DP>(Kt, st, s, col, half), qf[s], S);
@@ -734,11 +762,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const mi_attn_args p)
             // ds, over dp
 #pragma unroll
             for (int i = 0; i < 16; ++i) dP[i] = S[i] * (dP[i] - D);
-            if (masked) {
-                const uint32_t ok = at_allowed(p, keys, st, q - k0, half);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) dP[i] = (ok >> (8 * (i >> 2) + (i & 3))) & 1u ? dP[i] : 0.0f;
-            }
+            at_unattended(p, mask, (uint32_t)(keys >> (32 * st)), k0 + 32 * st, qw, q, len, half,
+                          [&](int i, bool on) __attribute__((always_inline)) { dP[i] = on ? dP[i] : 0.0f; });
             if constexpr (BIAS) {
                 if (near) {
                     float* const at = skew + col * 63 + 31 + 4 * half;
@@ -868,7 +893,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(const 
         if constexpr (BIAS) {
             if (head != bias_head) {
                 if (bias_head >= 0) at_sync();                         // the last head's vector has been read
-                at_fill_bias(p, head, p.scale_inv, vec);
+                at_fill_bias(p, head, p.scale_inv, 0.0f, vec);
                 bias_head = head;
             }
         }
@@ -878,13 +903,13 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(const 
         if (kw >= len || (p.causal && q0 + AT_KT - 1 < kw)) continue;
         const char* const Qt = lds + buf * 2 * TB;
         const char* const Dt = Qt + TB;
-        const bool edge = (p.causal && q0 < kw + 31) || q0 + AT_KT > len;   // rows that do not attend, or are none
         const int rlo = kw - (q0 + AT_KT - 1), rhi = kw + 31 - q0;
         const bool near = BIAS && rhi > -p.reach && rlo < p.reach;
         const float add = AtPScale<F16>::log2 + (BIAS && !near ? vec[rhi <= -p.reach ? 0 : 2 * R] * p.scale_log2 : 0.0f);
         const int at = key - q0 - 4 * half + R;
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
+            if (DP < 128 && (q0 + 32 * st >= len || (p.causal && q0 + 32 * st + 31 < kw))) continue;
             f32x16 S = at_first<F16>(near, vec + at - 32 * st, -1, at_rows<DP>(Qt, st, 0, col, half), kf[0]), dP = at_zero16();
 #pragma unroll
             for (int s = 1; s < DP / 16; ++s) S = at_mfma<F16>(at_rows<DP>(Qt, st, s, col, half), kf[s], S);
@@ -902,7 +927,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(const 
                     dP[i] = S[i] * ((dP[i] - Drs[e]) * AtPScale<F16>::down);
                 }
             }
-            if (edge) {
+            if ((p.causal && q0 + 32 * st < kw + 31) || q0 + 32 * st + 32 > len) {   // rows that do not attend, or are none
                 const int first = p.causal ? key - q0 - 32 * st - 4 * half : -AT_KT, end = len - q0 - 32 * st - 4 * half;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
