@@ -8,7 +8,6 @@
 // read with the same permutation of keys by the hardware transpose read, so no value crosses a lane).
 #include <float.h>
 #include <math.h>
-#include <stdlib.h>
 #include <atomic>
 #include <type_traits>
 #include "attention.h"
@@ -188,11 +187,11 @@ template <int DP, int NW> struct AtStage {
         off = (unsigned)(row0 * pitch + chunk);
         left = len - 1 - first;
     }
-    // the next 64 rows to lds_addr; mask: the key mask from the tile's first row on
-    __device__ __forceinline__ void issue(unsigned lds_addr, int wave, const int32_t* mask = nullptr)
+    // the next 64 rows to lds_addr; keys: which of them are keys
+    __device__ __forceinline__ void issue(unsigned lds_addr, int wave, uint64_t keys = ~0ull)
     {
         lds_addr += wave * 1024;
-        if (!mask && left >= AT_KT - 1) {
+        if (keys == ~0ull && left >= AT_KT - 1) {
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
                 at_dma16(off, at, lds_addr + (unsigned)(i * NW * 1024));
@@ -201,10 +200,9 @@ template <int DP, int NW> struct AtStage {
         } else {
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
-                int row = row0 + i * RPI * NW;
-                row = row < left ? row : left;
+                const int r = row0 + i * RPI * NW, row = r < left ? r : left;
                 const char* src = at + (int64_t)row * pitch + chunk;
-                if (mask && mask[row] == 0) src = reinterpret_cast<const char*>(&at_zero_chunk);
+                if (!((keys >> r) & 1)) src = reinterpret_cast<const char*>(&at_zero_chunk);
                 at_dma16(src, lds_addr + (unsigned)(i * NW * 1024));
             }
             at += (int64_t)AT_KT * pitch;
@@ -222,25 +220,79 @@ __device__ __forceinline__ void at_arrive(int ahead)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
+// everything outstanding has landed and been read, on every wave
+__device__ __forceinline__ void at_sync()
+{
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+// Which keys of a sequence the mask leaves, 64 a word.  The block reads the mask once, ahead of everything: so tiles without a key
+// are left out at the end (a padded batch's padding) and whole ones in front take the code without a mask.
+#define AT_WORDS 256                                  // tiles whose words are kept; later ones are asked for as they come
+struct AtKeys {
+    const int32_t* mask;                              // from the sequence's first row on, or NULL
+    const uint64_t* words;
+    int len, lane;
+    int full, some;                                   // leading tiles of 64 keys each; tiles up to the last one with a key
+    __device__ __forceinline__ uint64_t load(int t) const
+    {
+        const int key = t * AT_KT + lane;
+        return __builtin_amdgcn_ballot_w64(key < len && mask[key < len ? key : len - 1] != 0);
+    }
+    __device__ __forceinline__ uint64_t tile(int t) const
+    {
+        if (!mask) return ~0ull;
+        if (t >= AT_WORDS) return load(t);
+        const uint64_t w = words[t];
+        return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(w >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)w);
+    }
+    // waves: of the block, all of them call
+    __device__ __forceinline__ void init(const int32_t* key_mask, uint64_t* w, int start, int n, int kend, int wave, int waves, int l)
+    {
+        mask = key_mask ? key_mask + start : nullptr;
+        words = w;
+        len = n;
+        lane = l;
+        some = (kend + AT_KT - 1) / AT_KT;
+        full = some;
+        if (!mask) return;
+        const int tiles = some < AT_WORDS ? some : AT_WORDS;
+        for (int t = wave; t < tiles; t += waves) {
+            const uint64_t k = load(t);
+            if (lane == 0) w[t] = k;
+        }
+        at_sync();
+        full = 0;
+        int last = 0;
+        for (int t = 0; t < tiles; t += 64) {
+            const uint64_t k = t + lane < tiles ? w[t + lane] : 0;
+            const uint64_t whole = __builtin_amdgcn_ballot_w64(k == ~0ull), any = __builtin_amdgcn_ballot_w64(k != 0);
+            if (full == t) full += ~whole ? __builtin_ctzll(~whole) : 64;
+            if (any) last = t + 64 - __builtin_clzll(any);
+        }
+        if (some <= AT_WORDS) some = last;
+    }
+};
 // The K and V tiles of a sequence through NB pairs of buffers: tile t + NB - 1 is requested when every wave is done with tile t - 1.
 // (With two buffers a tile has one tile's computing to arrive, about 0.5 us at head size 32, and memory takes longer.)
 template <int DP, int NB> struct AtPipe {
     static constexpr int PAIR = 2 * AtTile<DP>::BYTES, BYTES = NB * PAIR, PER = 2 * AtStage<DP, 4>::NI;
     AtStage<DP, 4> a, b;
-    const int32_t* mask;
+    AtKeys* keys;
     unsigned lds0;
     int n, wave, buf;
     __device__ __forceinline__ void issue(int t, int slot)
     {
-        const int32_t* const m = mask ? mask + t * AT_KT : nullptr;
-        a.issue(lds0 + slot * PAIR, wave, m);
-        b.issue(lds0 + slot * PAIR + PAIR / 2, wave, m);
+        const uint64_t k = keys->tile(t);
+        a.issue(lds0 + slot * PAIR, wave, k);
+        b.issue(lds0 + slot * PAIR + PAIR / 2, wave, k);
     }
-    __device__ __forceinline__ void start(const char* lds, int tiles, const int32_t* key_mask, int w)
+    __device__ __forceinline__ void start(const char* lds, AtKeys* k, int w)
     {
         lds0 = (unsigned)(size_t)(const __attribute__((address_space(3))) char*)lds;
-        n = tiles;
-        mask = key_mask;
+        n = k->some;
+        keys = k;
         wave = w;
         buf = NB - 1;
 #pragma unroll
@@ -256,14 +308,6 @@ template <int DP, int NB> struct AtPipe {
         return buf * PAIR;
     }
 };
-// everything outstanding has landed and been read, on every wave
-__device__ __forceinline__ void at_sync()
-{
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
-
 // Operand rows straight from memory: row's chunks 2 s + half, s = 0 .. DP / 16 - 1, zero beyond head_dim.
 template <int DP>
 __device__ __forceinline__ void at_load_rows(u32x4 (&f)[DP / 16], const mi_attn_rows& x, int64_t token, int head, int hd, int half)
@@ -365,18 +409,12 @@ __device__ __forceinline__ void at_fill_bias(const mi_attn_args& p, int head, fl
     for (int i = threadIdx.x; i < 2 * R + 1; i += blockDim.x) vec[i] = at_bias(p, head, i - R, unit) + shift;
 }
 
-// Which of the 64 keys at k0 the mask leaves (bit = key - k0); the wave's lanes ask for one each.
-__device__ __forceinline__ uint64_t at_keys(const int32_t* mask, int k0, int len, int lane)
-{
-    const int key = k0 + lane;
-    return __builtin_amdgcn_ballot_w64(key < len && mask[key < len ? key : len - 1] != 0);
-}
 // Calls f(i, attended) for the registers of a block of scores, 32 keys from k on, one query a lane (register 4 g + i is key
-// k + 8 g + 4 half + i), where not all are attended; keys: the block's bits of at_keys, used where there is a mask.
+// k + 8 g + 4 half + i), where not all are attended; keys: the block's keys (all, without a mask).
 template <class F>
-__device__ __forceinline__ void at_unattended(const mi_attn_args& p, const int32_t* mask, uint32_t keys, int k, int qw, int q, int len, int half, F&& f)
+__device__ __forceinline__ void at_unattended(const mi_attn_args& p, bool mask, uint32_t keys, int k, int qw, int q, int len, int half, F&& f)
 {
-    if (k + 32 <= len && !(p.causal && k + 31 > qw) && !(mask && keys != 0xFFFFFFFFu)) return;
+    if (k + 32 <= len && !(p.causal && k + 31 > qw) && keys == 0xFFFFFFFFu) return;
     int lim = len - 1 - k;                                             // the last attended key but for the mask
     if (p.causal && q - k < lim) lim = q - k;
     lim -= 4 * half;
@@ -433,11 +471,14 @@ __global__ __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) void attn_fwd
     u32x4 qf[DP / 16];
     at_load_rows<DP>(qf, p.q, start + (q < len ? q : len - 1), head, p.hd, half);
     const int kvh = at_div(head, p.group_inv);
-    const int32_t* const mask = p.key_mask ? p.key_mask + start : nullptr;
+    __shared__ uint64_t words[AT_WORDS];
+    AtKeys keys;
+    keys.init(p.key_mask, words, start, len, kend, wave, 4, lane);
+    const bool mask = keys.mask != nullptr;
     AtPipe<DP, NB> pipe;
     pipe.a.init(p.k, start, 0, len, kvh, p.hd, wave, lane);
     pipe.b.init(p.v, start, 0, len, kvh, p.hd, wave, lane);
-    pipe.start(lds, (kend + AT_KT - 1) / AT_KT, mask, wave);
+    pipe.start(lds, &keys, wave);
     if constexpr (BIAS) at_fill_bias(p, head, AT_LOG2E, F16 ? 8.0f : 0.0f, vec);
 
     f32x16 O[DP / 32];
@@ -458,7 +499,7 @@ __global__ __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) void attn_fwd
         constexpr bool MASKED = decltype(masked_)::value;
         constexpr int FORM = decltype(form_)::value;
         const int kw = k0 + 32 * s0;
-        const uint64_t keys = MASKED && mask ? at_keys(mask, k0, len, lane) : 0;
+        const uint64_t on = MASKED ? keys.tile(k0 / AT_KT) : 0;
         const float less = BIAS ? vec[kw < qw ? 0 : 2 * R] - m : -REF0 - m;
         f32x16 S[NS];
 #pragma unroll
@@ -474,7 +515,7 @@ __global__ __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) void attn_fwd
                 lim = len - 1 - kw - 32 * n;
                 if (p.causal && q - kw - 32 * n < lim) lim = q - kw - 32 * n;
                 lim -= 4 * half;
-                ok = (uint32_t)(keys >> (32 * (s0 + n))) >> (4 * half);
+                ok = (uint32_t)(on >> (32 * (s0 + n))) >> (4 * half);
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -529,8 +570,10 @@ __global__ __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) void attn_fwd
     if (qw < len) {
         const int end = p.causal && qw + 32 < kend ? qw + 32 : kend;
         live = end <= 32 * s0 ? 0 : (end - 32 * s0 + AT_KT - 1) / AT_KT;
-        plain = mask || lim < 32 * (NS + s0) ? 0 : (lim - 32 * (NS + s0)) / AT_KT + 1;
+        if (live > all) live = all;
+        plain = lim < 32 * (NS + s0) ? 0 : (lim - 32 * (NS + s0)) / AT_KT + 1;
         if (plain > live) plain = live;
+        if (mask && plain > keys.full) plain = keys.full;
         if constexpr (BIAS) {
             const int x = qw - p.reach - 32 * (NS + s0) + 1, y = qw + 31 + p.reach - 32 * s0;   // before: k0 <= x; behind: k0 >= y
             far0 = x < 0 ? 0 : x / AT_KT + 1;
@@ -615,7 +658,7 @@ __global__ __launch_bounds__(256, 2) void attn_delta_kernel(const mi_attn_args p
     const int qw = tile * BM + wave * 32, q = qw + col;
     const int kend = p.causal ? (tile * BM + BM < len ? tile * BM + BM : len) : len;
     const int64_t tok = start + (q < len ? q : len - 1);
-    const int32_t* const mask = p.key_mask ? p.key_mask + start : nullptr;
+    const bool mask = p.key_mask != nullptr;
     u32x4 df[DP / 16], qf[DP / 16];                                    // qf: rows of out, or of q
     at_load_rows<DP>(df, p.dout, tok, head, p.hd, half);
     float nl = p.lse[(int64_t)head * p.tokens + tok] * AT_LOG2E;
@@ -633,16 +676,19 @@ __global__ __launch_bounds__(256, 2) void attn_delta_kernel(const mi_attn_args p
         c = half == 0 ? 1.0f : 0.0f;
     } else {
         at_load_rows<DP>(qf, p.q, tok, head, p.hd, half);
+        __shared__ uint64_t words[AT_WORDS];
+        AtKeys keys;
+        keys.init(p.key_mask, words, start, len, kend, wave, 4, lane);
         AtPipe<DP, NB> pipe;
         pipe.a.init(p.k, start, 0, len, at_div(head, p.group_inv), p.hd, wave, lane);
         pipe.b.init(p.v, start, 0, len, at_div(head, p.group_inv), p.hd, wave, lane);
-        pipe.start(lds, (kend + AT_KT - 1) / AT_KT, mask, wave);
+        pipe.start(lds, &keys, wave);
         if constexpr (BIAS) at_fill_bias(p, head, AT_LOG2E, 0.0f, vec);
         const int R = p.reach + AT_PAD;
-        for (int k0 = 0; k0 < kend; k0 += AT_KT) {
+        for (int k0 = 0; k0 < pipe.n * AT_KT; k0 += AT_KT) {
             const char* const Kt = lds + pipe.next(k0 / AT_KT);
             if (qw >= len || (p.causal && k0 > qw + 31)) continue;
-            const uint64_t keys = mask ? at_keys(mask, k0, len, lane) : 0;
+            const uint64_t on = keys.tile(k0 / AT_KT);
             const int rlo = k0 - (qw + 31), rhi = k0 + AT_KT - 1 - qw;
             const bool near = BIAS && rhi > -p.reach && rlo < p.reach;
             const float far = BIAS && !near ? vec[rhi <= -p.reach ? 0 : 2 * R] - nl : -nl;
@@ -662,9 +708,9 @@ __global__ __launch_bounds__(256, 2) void attn_delta_kernel(const mi_attn_args p
 #pragma unroll
                     for (int i = 0; i < 16; ++i) S[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], p.scale_log2, far));
                 }
-                at_unattended(p, mask, (uint32_t)(keys >> (32 * st)), k0 + 32 * st, qw, q, len, half, [&](int i, bool on) __attribute__((always_inline)) {
-                    S[i] = on ? S[i] : 0.0f;
-                    dP[i] = on ? dP[i] : 0.0f;
+                at_unattended(p, mask, (uint32_t)(on >> (32 * st)), k0 + 32 * st, qw, q, len, half, [&](int i, bool yes) __attribute__((always_inline)) {
+                    S[i] = yes ? S[i] : 0.0f;
+                    dP[i] = yes ? dP[i] : 0.0f;
                 });
                 float a1 = 0.0f, c1 = 0.0f;                            // (short chains: a long row's sums stay exact to fp32's last bits)
 #pragma unroll
@@ -715,11 +761,14 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const mi_attn_args p)
     const int kend = p.causal ? (tile * BM + BM < len ? tile * BM + BM : len) : len;
     const int kvh = at_div(head, p.group_inv);
 
-    const int32_t* const mask = p.key_mask ? p.key_mask + start : nullptr;
+    __shared__ uint64_t words[AT_WORDS];
+    AtKeys keys;
+    keys.init(p.key_mask, words, start, len, kend, wave, 4, lane);
+    const bool mask = keys.mask != nullptr;
     AtPipe<DP, NB> pipe;
     pipe.a.init(p.k, start, 0, len, kvh, p.hd, wave, lane);
     pipe.b.init(p.v, start, 0, len, kvh, p.hd, wave, lane);
-    pipe.start(lds, (kend + AT_KT - 1) / AT_KT, mask, wave);
+    pipe.start(lds, &keys, wave);
 
     u32x4 qf[DP / 16], df[DP / 16];
     const int64_t tok = start + (q < len ? q : len - 1);
@@ -741,10 +790,10 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const mi_attn_args p)
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) dQ[dt] = at_zero16();
 
-    for (int k0 = 0; k0 < kend; k0 += AT_KT) {
+    for (int k0 = 0; k0 < pipe.n * AT_KT; k0 += AT_KT) {
         const char* const Kt = lds + pipe.next(k0 / AT_KT);
         if (qw >= len || (p.causal && k0 > qw + 31)) continue;
-        const uint64_t keys = mask ? at_keys(mask, k0, len, lane) : 0;
+        const uint64_t on = keys.tile(k0 / AT_KT);
         const int rlo = k0 - (qw + 31), rhi = k0 + AT_KT - 1 - qw;
         const bool near = BIAS && rhi > -p.reach && rlo < p.reach;
         const float far = BIAS && !near ? __builtin_fmaf(vec[rhi <= -p.reach ? 0 : 2 * R], p.scale_log2, -nl) : -nl;
@@ -762,8 +811,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const mi_attn_args p)
             // ds, over dp
 #pragma unroll
             for (int i = 0; i < 16; ++i) dP[i] = S[i] * (dP[i] - D);
-            at_unattended(p, mask, (uint32_t)(keys >> (32 * st)), k0 + 32 * st, qw, q, len, half,
-                          [&](int i, bool on) __attribute__((always_inline)) { dP[i] = on ? dP[i] : 0.0f; });
+            at_unattended(p, mask, (uint32_t)(on >> (32 * st)), k0 + 32 * st, qw, q, len, half,
+                          [&](int i, bool yes) __attribute__((always_inline)) { dP[i] = yes ? dP[i] : 0.0f; });
             if constexpr (BIAS) {
                 if (near) {
                     float* const at = skew + col * 63 + 31 + 4 * half;
@@ -1032,7 +1081,7 @@ static int at_lds(size_t bytes)
     MI_HIP(hipGetDevice(&dev));
     const uint64_t bit = 1ull << (dev & 63);
     if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return MI_OK;
-    MI_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+    MI_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, 156 * 1024));   // (160 KB less the mask words)
     if (dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
     return MI_OK;
 }
@@ -1053,8 +1102,11 @@ static int launch_fwd(hipStream_t st, mi_attn_args& a)
 template <int DP, bool F16>
 static int launch_fwd(hipStream_t st, mi_attn_args& a)
 {
-    static const int force = getenv("AT_KS") ? atoi(getenv("AT_KS")) : 0;
-    const bool split = force ? force == 2 : false;
+    // Two waves to a query where 128-row blocks are fewer than four to a CU: 432 blocks (2 causal documents up to 4,099, 8 heads of
+    // 64, bias) 76 -> 56 us, 520 (8,191, 8 heads of 128) 178 -> 160 us; 1,500 blocks (prompts up to 2,039, 32 heads of 128) 92 us
+    // either way, 2,048 (16,384, 16 heads of 128) 1,066 -> 1,243 us, 8,900 (chunks up to 256, 12 heads of 32) 67 -> 83 us.
+    const int64_t blocks = (int64_t)a.heads * (a.tokens / 128 + a.nseq);
+    const bool split = blocks < 1024;
     if (a.table) return split ? launch_fwd<DP, F16, true, 2>(st, a) : launch_fwd<DP, F16, true, 1>(st, a);
     return split ? launch_fwd<DP, F16, false, 2>(st, a) : launch_fwd<DP, F16, false, 1>(st, a);
 }
