@@ -875,7 +875,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const mi_attn_args p)
 // head and tile would leave CUs idle the group's heads are shared out over `splits` blocks, whose fp32 sums attn_join_kernel
 // adds in the heads' order.
 template <int DP, bool F16, bool BIAS>
-__global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(const mi_attn_args p)
+__global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const mi_attn_args p)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     constexpr int BM = 128, TB = AtTile<DP>::BYTES, NB = AT_BUFFERS(DP), PER = 2 * AtStage<DP, 4>::NI + 1;
@@ -958,7 +958,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(const 
         const int at = key - q0 - 4 * half + R;
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
-            if (DP < 128 && (q0 + 32 * st >= len || (p.causal && q0 + 32 * st + 31 < kw))) continue;
+            if ((q0 + 32 * st >= len || (p.causal && q0 + 32 * st + 31 < kw))) continue;
             f32x16 S = at_first<F16>(near, vec + at - 32 * st, -1, at_rows<DP>(Qt, st, 0, col, half), kf[0]), dP = at_zero16();
 #pragma unroll
             for (int s = 1; s < DP / 16; ++s) S = at_mfma<F16>(at_rows<DP>(Qt, st, s, col, half), kf[s], S);
@@ -1014,6 +1014,177 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(const 
             at_store_part<DP>(p.parts_kv, ((int64_t)(2 * share) * p.tokens + start + key) * (p.heads / p.group) + kvh, p.hd, half, dK, p.scale);
             at_store_part<DP>(p.parts_kv, ((int64_t)(2 * share + 1) * p.tokens + start + key) * (p.heads / p.group) + kvh, p.hd, half, dV, AtPScale<F16>::down);
         }
+    }
+}
+
+// The same at head sizes above 64, where dK, dV, K and V of 32 keys (192 registers and what the products need) leave a SIMD one wave,
+// which nothing overlaps with: 1 x 8,191 causal, 8 heads of 128, 412 us where this form takes @PAIR@ us.  Eight waves, two to 32 keys: wave A
+// makes S and P and sums dV, wave B makes dP and dS and sums dK.  P goes from A to B through LDS in fp32, each register to the same
+// lane's; a SIMD has one wave of either kind, so one's exponentials run beside the other's products.  Two barriers a tile: it has
+// landed, P is there.
+template <bool F16, bool BIAS>
+__global__ __launch_bounds__(512, 2) void attn_dkv_pair_kernel(const mi_attn_args p)
+{
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    constexpr int DP = 128, BM = 128, TB = AtTile<DP>::BYTES, NB = 2, PER = 2 * AtStage<DP, 8>::NI + 1;
+    float* const rowv = reinterpret_cast<float*>(lds + NB * 2 * TB);   // [NB][lse in log2 units | D][64]
+    float4* const pass = reinterpret_cast<float4*>(rowv + NB * 128);   // [4 pairs][8][64 lanes]
+    float* const vec = reinterpret_cast<float*>(pass + 4 * 8 * 64);
+    int kvh, t, start, len, tile;
+    bool tail;
+    if (!at_work(p, kvh, t) || !at_find<BM>(p, t, start, len, tile, tail)) return;
+    const int unit = kvh, heads = p.share_heads;                       // (units are key heads x shares)
+    kvh = at_div(unit, p.splits_inv);
+    const int share = unit - kvh * p.splits;
+    const int head0 = kvh * p.group + share * heads;
+    if (tail) {
+        if (share != 0) return;
+        const int n = len - tile * BM < BM ? len - tile * BM : BM;
+        at_zero_rows(p.dk, start + tile * BM, n, kvh, p.hd);
+        at_zero_rows(p.dv, start + tile * BM, n, kvh, p.hd);
+        return;
+    }
+    if (tile * BM >= len) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, half = lane >> 5, pair = wave & 3;
+    const bool first = wave < 4;                                       // wave A
+    const int kw = tile * BM + pair * 32, key = kw + col;
+    const int64_t ktok = start + (key < len ? key : len - 1);
+    u32x4 wf[DP / 16];                                                 // K or V
+    at_load_rows<DP>(wf, first ? p.k : p.v, ktok, kvh, p.hd, half);
+    const bool on = key < len && (!p.key_mask || p.key_mask[ktok] != 0);
+
+    const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds;
+    const int qfirst = p.causal ? tile * BM / AT_KT * AT_KT : 0;       // earlier queries attend no key of this block
+    const int nq = (len - qfirst + AT_KT - 1) / AT_KT, n = nq * heads;
+    AtStage<DP, 8> qs, ds;
+    int ihead = head0 - 1, iq = nq;                                    // the tile requested last: its head, its number
+    const float* rows = nullptr;
+    auto issue = [&](int slot) __attribute__((always_inline)) {
+        if (++iq >= nq) {
+            iq = 0;
+            ++ihead;
+            qs.init(p.q, start, qfirst, len, ihead, p.hd, wave, lane);
+            ds.init(p.dout, start, qfirst, len, ihead, p.hd, wave, lane);
+            rows = (wave & 1 ? p.delta : p.lse2) + (int64_t)ihead * p.tokens + start;
+        }
+        qs.issue(lds0 + slot * 2 * TB, wave);
+        ds.issue(lds0 + slot * 2 * TB + TB, wave);
+        // 64 values of each row vector: even waves the log-sum-exp, odd ones D (the others the same again)
+        const int q = qfirst + iq * AT_KT + lane;
+        at_dma4(rows + (q < len ? q : len - 1), lds0 + NB * 2 * TB + (unsigned)(slot * 128 + (wave & 1) * 64) * 4);
+    };
+    f32x16 acc[DP / 32];                                               // dV^T or dK^T
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = at_zero16();
+    issue(0);
+    const int R = p.reach + AT_PAD;
+    int bias_head = -1, head = head0, q0 = qfirst - AT_KT, buf = NB - 1;
+    // the next tile has landed; the one behind it is requested
+    auto next = [&](int it) __attribute__((always_inline)) {
+        q0 += AT_KT;
+        if (q0 >= len) {
+            q0 = qfirst;
+            ++head;
+        }
+        if constexpr (BIAS) {
+            if (head != bias_head) {
+                if (bias_head >= 0) at_sync();                         // the last head's vector has been read
+                at_fill_bias(p, head, AT_LOG2E, AtPScale<F16>::log2, vec);
+                bias_head = head;
+            }
+        }
+        at_arrive<PER>(0);
+        if (it + 1 < n) issue(buf);
+        buf ^= 1;
+        return lds + buf * 2 * TB;
+    };
+    auto there = [&]() __attribute__((always_inline)) {                // what a wave wrote to LDS is there for the others
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    auto sum_up = [&](const char* rows_t, const f32x16 (&X)[2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+            u32x4 f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = at_pack2<F16>(X[kk >> 1][8 * (kk & 1) + 2 * i], X[kk >> 1][8 * (kk & 1) + 2 * i + 1]);
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = at_mfma<F16>(at_cols<DP>(rows_t, kk, dt, lane), f, acc[dt]);
+        }
+    };
+    float4* const mine = pass + pair * 8 * 64 + lane;
+    if (first) {
+        for (int it = 0; it < n; ++it) {
+            const char* const Qt = next(it);
+            const bool idle = kw >= len || (p.causal && q0 + AT_KT - 1 < kw);
+            f32x16 S[2];
+            if (!idle) {
+#pragma unroll
+                for (int st = 0; st < 2; ++st)
+#pragma unroll
+                    for (int s = 0; s < DP / 16; ++s) S[st] = at_mfma<F16>(at_rows<DP>(Qt, st, s, col, half), wf[s], s == 0 ? at_zero16() : S[st]);
+                const int rlo = kw - (q0 + AT_KT - 1), rhi = kw + 31 - q0;
+                const bool near = BIAS && rhi > -p.reach && rlo < p.reach;
+                const float add = BIAS ? (near ? 0.0f : vec[rhi <= -p.reach ? 0 : 2 * R]) : AtPScale<F16>::log2;
+                const float* const bv = vec + (key - q0 - 4 * half + R);
+                const bool edge = (p.causal && q0 < kw + 31) || q0 + AT_KT > len;      // rows that do not attend, or are none
+                const int lo = p.causal ? key - q0 - 4 * half : -AT_KT, hi = len - q0 - 4 * half;
+#pragma unroll
+                for (int st = 0; st < 2; ++st) {
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const float4 nl = *reinterpret_cast<const float4*>(rowv + buf * 128 + 32 * st + 8 * g + 4 * half);
+                        const float nls[4] = {nl.x, nl.y, nl.z, nl.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int i = 4 * g + e, r = 32 * st + 8 * g + e;
+                            const float b = BIAS && near ? bv[-r] : add;
+                            S[st][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[st][i], p.scale_log2, b - nls[e]));
+                            if (edge) S[st][i] = r >= lo && r < hi ? S[st][i] : 0.0f;
+                        }
+                        mine[(4 * st + g) * 64] = make_float4(S[st][4 * g], S[st][4 * g + 1], S[st][4 * g + 2], S[st][4 * g + 3]);
+                    }
+                }
+            }
+            there();
+            if (!idle) sum_up(Qt + TB, S);
+        }
+    } else {
+        for (int it = 0; it < n; ++it) {
+            const char* const Qt = next(it);
+            const bool idle = kw >= len || (p.causal && q0 + AT_KT - 1 < kw);
+            f32x16 dP[2];
+            if (!idle) {
+#pragma unroll
+                for (int st = 0; st < 2; ++st)
+#pragma unroll
+                    for (int s = 0; s < DP / 16; ++s) dP[st] = at_mfma<F16>(at_rows<DP>(Qt + TB, st, s, col, half), wf[s], s == 0 ? at_zero16() : dP[st]);
+            }
+            there();
+            if (!idle) {
+#pragma unroll
+                for (int st = 0; st < 2; ++st)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const float4 Dr = *reinterpret_cast<const float4*>(rowv + buf * 128 + 64 + 32 * st + 8 * g + 4 * half), P = mine[(4 * st + g) * 64];
+                        const float Drs[4] = {Dr.x, Dr.y, Dr.z, Dr.w}, Ps[4] = {P.x, P.y, P.z, P.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) dP[st][4 * g + e] = Ps[e] * ((dP[st][4 * g + e] - Drs[e]) * AtPScale<F16>::down);
+                    }
+                sum_up(Qt, dP);
+            }
+        }
+    }
+    if (key < len) {
+        if (!on) {                                                     // a masked key (the products above ran on its column alone)
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = at_zero16();
+        }
+        const float f = first ? AtPScale<F16>::down : p.scale;
+        if (p.splits == 1) at_store_row<DP, F16>(first ? p.dv : p.dk, start + key, kvh, p.hd, half, acc, f);
+        else at_store_part<DP>(p.parts_kv, ((int64_t)(2 * share + (first ? 1 : 0)) * p.tokens + start + key) * at_div(p.heads, p.group_inv) + kvh, p.hd, half, acc, f);
     }
 }
 
@@ -1177,13 +1348,25 @@ static int launch_bwd(hipStream_t st, mi_attn_args& a)
     }
     const dim3 grid = at_schedule(&a, a.heads / a.group * a.splits, 128);
     if (grid.x == 0) return MI_OK;
-    const size_t smem = AT_BUFFERS(DP) * (2 * AtTile<DP>::BYTES + 512) + (a.table ? (size_t)(2 * (a.reach + AT_PAD) + 1) * 4 : 0);
-    if (a.table) {
-        MI_TRY((at_lds<&attn_dkv_kernel<DP, F16, true>>(smem)));
-        attn_dkv_kernel<DP, F16, true><<<grid, 256, smem, st>>>(a);
+    const size_t bias = a.table ? (size_t)(2 * (a.reach + AT_PAD) + 1) * 4 : 0;
+    if constexpr (DP == 128) {
+        const size_t smem = 2 * (2 * AtTile<DP>::BYTES + 512) + 4 * 8 * 64 * 16 + bias;
+        if (a.table) {
+            MI_TRY((at_lds<&attn_dkv_pair_kernel<F16, true>>(smem)));
+            attn_dkv_pair_kernel<F16, true><<<grid, 512, smem, st>>>(a);
+        } else {
+            MI_TRY((at_lds<&attn_dkv_pair_kernel<F16, false>>(smem)));
+            attn_dkv_pair_kernel<F16, false><<<grid, 512, smem, st>>>(a);
+        }
     } else {
-        MI_TRY((at_lds<&attn_dkv_kernel<DP, F16, false>>(smem)));
-        attn_dkv_kernel<DP, F16, false><<<grid, 256, smem, st>>>(a);
+        const size_t smem = AT_BUFFERS(DP) * (2 * AtTile<DP>::BYTES + 512) + bias;
+        if (a.table) {
+            MI_TRY((at_lds<&attn_dkv_kernel<DP, F16, true>>(smem)));
+            attn_dkv_kernel<DP, F16, true><<<grid, 256, smem, st>>>(a);
+        } else {
+            MI_TRY((at_lds<&attn_dkv_kernel<DP, F16, false>>(smem)));
+            attn_dkv_kernel<DP, F16, false><<<grid, 256, smem, st>>>(a);
+        }
     }
     MI_HIP(hipGetLastError());
     if (a.splits > 1) {
