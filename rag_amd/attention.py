@@ -54,6 +54,15 @@ def _config(heads, kv_heads, hd, dtype, causal, scale, buckets, max_distance, bi
     return AttentionConfig(heads, kv_heads, hd, dtype, int(bool(causal)), 1, float(scale), buckets, int(max_distance), int(bool(bidirectional)))
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace(heads, kv_heads, hd, buckets, max_distance, bidirectional, tokens, nseq, packed) -> int:
+    """Words of workspace of the backward pass."""
+    cfg = AttentionConfig(heads, kv_heads, hd, _capi.DTYPE_BF16, 0, 1, 1.0, buckets, max_distance, bidirectional)
+    need = ctypes.c_size_t()
+    _capi.check(_capi.load().mi_attention_backward_workspace(cfg, tokens, nseq, packed, ctypes.byref(need)))
+    return (max(need.value, 4) + 3) // 4
+
+
 def _setup(q, k, v, offsets, causal, scale, key_mask, bias_table, max_distance, bidirectional):
     """(config, tokens, nseq, addresses of offsets, key_mask, bias_table) after the checks."""
     z, device = q.shape, q.device
@@ -141,10 +150,8 @@ def packed_attention_backward(dout, q, k, v, out, lse, offsets=None, *, causal: 
             _rows("dout", dout, z, dtype, device))
     dq, dk, dv = q.new_empty(z), k.new_empty(zk), v.new_empty(zk)
     dtable = bias_table.new_empty(bias_table.shape) if bias_table is not None else None
-    lib, need = _capi.load(), ctypes.c_size_t()
-    _capi.check(lib.mi_attention_backward_workspace(cfg, tokens, nseq, offsets is not None, ctypes.byref(need)))
-    work = q.new_empty((max(need.value, 4) + 3) // 4, dtype=_F32)
-    _capi.check(lib.mi_attention_backward_dev(_capi.get_ctx(device.index), cfg, tokens, nseq, off, mask, rows[0], rows[1], rows[2], table, rows[3],
+    work = q.new_empty(_workspace(heads, zk[-2], z[-1], cfg.num_buckets, cfg.max_distance, cfg.bidirectional, tokens, nseq, offsets is not None), dtype=_F32)
+    _capi.check(_capi.load().mi_attention_backward_dev(_capi.get_ctx(device.index), cfg, tokens, nseq, off, mask, rows[0], rows[1], rows[2], table, rows[3],
                                               lse.data_ptr(), rows[4], _rows("dq", dq, z, dtype, device), _rows("dk", dk, zk, dtype, device),
                                               _rows("dv", dv, zk, dtype, device), dtable.data_ptr() if dtable is not None else None, work.data_ptr(),
                                               work.numel() * 4, _capi.stream_arg(device)))

@@ -24,6 +24,7 @@ struct mi_attn_args {
     float* parts_kv = nullptr;            // backward workspace [splits][dk | dv][tokens][key heads][hd], where splits > 1
     int splits = 1, share_heads = 1;      // shares of a group's query heads in the dK / dV kernel
     float* dtable = nullptr;              // [buckets][heads]
+    int dq_tiles = 0, dtable_x = 0;       // `partial`'s tiles; where in the dK / dV grid's x (/ 8) its blocks begin
     int64_t tokens = 0;
     int nseq = 0, uniform_len = 0;
     int heads = 0, group = 1, hd = 0;     // group = query heads per key head

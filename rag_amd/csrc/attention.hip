@@ -643,11 +643,11 @@ template <bool F16> struct AtPScale { static constexpr float log2 = F16 ? 12.0f 
 // the table's gradient, a sum of many ds that nearly cancel.  So with a bias, for rows of up to 128 keys, and for up to 512 where
 // a mask may leave few of them, the sum is made from the scores, in fp32; other rows take the dot product.  Also writes the rows'
 // log-sum-exp the way the other two kernels take it: in log2 units, +inf for a row that attends nothing.
-template <int DP, bool F16, bool BIAS>
+template <int DP, bool F16, bool BIAS, int KS>
 __global__ __launch_bounds__(256, 2) void attn_delta_kernel(const mi_attn_args p)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    constexpr int BM = 128, TB = AtTile<DP>::BYTES, NB = AT_BUFFERS(DP);
+    constexpr int BM = 128 / KS, TB = AtTile<DP>::BYTES, NB = AT_BUFFERS(DP);
     float* const vec = reinterpret_cast<float*>(lds + NB * 2 * TB);
     int head, t, start, len, tile;
     bool tail;
@@ -655,7 +655,7 @@ __global__ __launch_bounds__(256, 2) void attn_delta_kernel(const mi_attn_args p
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     if (p.causal) tile = (len + BM - 1) / BM - 1 - tile;
-    const int qw = tile * BM + wave * 32, q = qw + col;
+    const int qw = tile * BM + (KS == 1 ? wave : wave & 1) * 32, q = qw + col, s0 = KS == 1 ? 0 : wave >> 1;   // as in attn_fwd_kernel
     const int kend = p.causal ? (tile * BM + BM < len ? tile * BM + BM : len) : len;
     const int64_t tok = start + (q < len ? q : len - 1);
     const bool mask = p.key_mask != nullptr;
@@ -674,6 +674,7 @@ __global__ __launch_bounds__(256, 2) void attn_delta_kernel(const mi_attn_args p
                 a = __builtin_fmaf(at_hi<F16>(df[s][j]), at_hi<F16>(qf[s][j]), a);
             }
         c = half == 0 ? 1.0f : 0.0f;
+        if (s0 > 0) a = c = 0.0f;                                      // (the other wave of the row has it)
     } else {
         at_load_rows<DP>(qf, p.q, tok, head, p.hd, half);
         __shared__ uint64_t words[AT_WORDS];
@@ -687,14 +688,14 @@ __global__ __launch_bounds__(256, 2) void attn_delta_kernel(const mi_attn_args p
         const int R = p.reach + AT_PAD;
         for (int k0 = 0; k0 < pipe.n * AT_KT; k0 += AT_KT) {
             const char* const Kt = lds + pipe.next(k0 / AT_KT);
-            if (qw >= len || (p.causal && k0 > qw + 31)) continue;
+            if (qw >= len || (p.causal && k0 + 32 * s0 > qw + 31)) continue;
             const uint64_t on = keys.tile(k0 / AT_KT);
             const int rlo = k0 - (qw + 31), rhi = k0 + AT_KT - 1 - qw;
             const bool near = BIAS && rhi > -p.reach && rlo < p.reach;
             const float far = BIAS && !near ? vec[rhi <= -p.reach ? 0 : 2 * R] - nl : -nl;
             const float* const bv = vec + (k0 + 4 * half - q + R);
 #pragma unroll
-            for (int st = 0; st < 2; ++st) {
+            for (int st = s0; st < (KS == 1 ? 2 : s0 + 1); ++st) {
                 if (st > 0 && (k0 + 32 >= kend || (p.causal && k0 + 32 > qw + 31))) break;
                 f32x16 S = at_zero16(), dP = at_zero16();
 #pragma unroll
@@ -722,6 +723,18 @@ __global__ __launch_bounds__(256, 2) void attn_delta_kernel(const mi_attn_args p
     }
     a += at_other_half(a);
     c += at_other_half(c);
+    if constexpr (KS == 2) {
+        at_sync();
+        float* const x = reinterpret_cast<float*>(lds) + (wave & 1) * 128 + lane;
+        if (wave >= 2) {
+            x[0] = a;
+            x[64] = c;
+        }
+        at_sync();
+        if (wave >= 2) return;
+        a += x[0];
+        c += x[64];
+    }
     if (half == 0 && q < len) {
         p.delta[(int64_t)head * p.tokens + tok] = c == 0.0f ? a : a / c;
         p.lse2[(int64_t)head * p.tokens + tok] = nl;
@@ -736,11 +749,11 @@ __global__ __launch_bounds__(256, 2) void attn_delta_kernel(const mi_attn_args p
 // image in LDS, element (key, query) at [query][key - query + 31], so that lane l finds a diagonal in column l (the positions a row
 // never writes hold the zeros they started with); the 63 sums are added to the wave's vector over r.  A tile of one bucket adds
 // in registers.  Every sum has one owner and a fixed order.  @DQ_BIAS@
-template <int DP, bool F16, bool BIAS>
+template <int DP, bool F16, bool BIAS, int KS>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const mi_attn_args p)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    constexpr int BM = 128, TB = AtTile<DP>::BYTES, NB = AT_DQ_BUFFERS(DP, BIAS);
+    constexpr int BM = 128 / KS, TB = AtTile<DP>::BYTES, NB = AT_DQ_BUFFERS(DP, BIAS);
     const int R = p.reach + AT_PAD, nvec = 2 * R + 1;
     float* const skew0 = reinterpret_cast<float*>(lds + NB * 2 * TB);       // BIAS: [4][32][64], the waves' images
     float* const vec = skew0 + 4 * 32 * 64;                            // the bias over r
@@ -757,7 +770,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const mi_attn_args p)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     if (p.causal) tile = (len + BM - 1) / BM - 1 - tile;
-    const int qw = tile * BM + wave * 32, q = qw + col;
+    const int qw = tile * BM + (KS == 1 ? wave : wave & 1) * 32, q = qw + col, s0 = KS == 1 ? 0 : wave >> 1;   // as in attn_fwd_kernel
     const int kend = p.causal ? (tile * BM + BM < len ? tile * BM + BM : len) : len;
     const int kvh = at_div(head, p.group_inv);
 
@@ -792,14 +805,14 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const mi_attn_args p)
 
     for (int k0 = 0; k0 < pipe.n * AT_KT; k0 += AT_KT) {
         const char* const Kt = lds + pipe.next(k0 / AT_KT);
-        if (qw >= len || (p.causal && k0 > qw + 31)) continue;
+        if (qw >= len || (p.causal && k0 + 32 * s0 > qw + 31)) continue;
         const uint64_t on = keys.tile(k0 / AT_KT);
         const int rlo = k0 - (qw + 31), rhi = k0 + AT_KT - 1 - qw;
         const bool near = BIAS && rhi > -p.reach && rlo < p.reach;
         const float far = BIAS && !near ? __builtin_fmaf(vec[rhi <= -p.reach ? 0 : 2 * R], p.scale_log2, -nl) : -nl;
         const float* const bv = vec + (k0 + 4 * half - q + R);
 #pragma unroll
-        for (int st = 0; st < 2; ++st) {
+        for (int st = s0; st < (KS == 1 ? 2 : s0 + 1); ++st) {
             if (st > 0 && (k0 + 32 >= kend || (p.causal && k0 + 32 > qw + 31))) break;
             f32x16 S = at_first<F16>(near, bv + 32 * st, 1, at_rows<DP>(Kt, st, 0, col, half), qf[0]), dP = at_zero16();
 #pragma unroll
@@ -840,28 +853,50 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const mi_attn_args p)
             }
         }
     }
-    if (q < len) at_store_row<DP, F16>(p.dq, start + q, head, p.hd, half, dQ, p.scale);
+    if constexpr (KS == 2) {
+        at_sync();
+        float* const x = reinterpret_cast<float*>(lds) + (wave & 1) * (DP / 2) * 64 + lane;
+        if (wave >= 2) {
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[(16 * dt + i) * 64] = dQ[dt][i];
+        }
+        at_sync();
+        if (wave < 2) {
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) dQ[dt][i] += x[(16 * dt + i) * 64];
+        }
+    }
+    if (q < len && (KS == 1 || wave < 2)) at_store_row<DP, F16>(p.dq, start + q, head, p.hd, half, dQ, p.scale);
     if constexpr (BIAS) {
-        // lane b of each wave sums the wave's diagonals of bucket b, then one wave adds the waves
+        // The diagonals of a wave by buckets: those of the outermost buckets across the lanes (one-sided, whatever is ahead counts as
+        // distance 0), then lane b those of bucket b, four at a time.  One lane after another over the outermost ones took 3 us a block.
+        for (int d = p.reach + lane; d <= R; d += 64) farS[0] += dvec[R - d];
+        for (int d = (p.two_sided ? p.reach : 1) + lane; d <= R; d += 64) farS[1] += dvec[R + d];
 #pragma unroll
         for (int s = 32; s > 0; s >>= 1) {
             farS[0] += __shfl_xor(farS[0], s, 64);
             farS[1] += __shfl_xor(farS[1], s, 64);
         }
-        if (lane == 0) {
-            dvec[0] += farS[0];
-            dvec[2 * R] += farS[1];
-        }
         float sum = 0.0f;
         if (lane < p.buckets) {
             const bool ahead = p.two_sided && lane >= p.side;          // r > 0
             const int i = ahead ? lane - p.side : lane;
-            int lo = i < p.exact ? i : i == p.exact ? p.exact : p.border[i - p.exact - 1];           // distances lo .. hi
-            int hi = i < p.exact ? i : i - p.exact < p.nborder ? p.border[i - p.exact] - 1 : R;
+            int lo = i <= p.exact ? i : p.border[i - p.exact - 1];     // distances lo .. hi
+            const int hi = i < p.exact ? i : (i - p.exact < p.nborder ? p.border[i - p.exact] : p.reach) - 1;
             if (ahead && lo == 0) lo = 1;                              // distance 0 is not ahead
-            for (int d = lo; d <= hi; ++d) sum += dvec[ahead ? R + d : R - d];
-            if (!p.two_sided && lane == 0)
-                for (int d = 1; d <= R; ++d) sum += dvec[R + d];       // one-sided: whatever is ahead counts as distance 0
+            const float* const at = dvec + R;
+            const int sign = ahead ? 1 : -1;
+            float part4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int d = lo; d <= hi; d += 4)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) part4[e] += d + e <= hi ? at[sign * (d + e <= hi ? d + e : hi)] : 0.0f;
+            sum = (part4[0] + part4[1]) + (part4[2] + part4[3]);
+            if (lane == p.side - 1) sum += farS[0];
+            if (lane == (p.two_sided ? p.buckets - 1 : 0)) sum += farS[1];
         }
         at_sync();
         skew0[wave * 64 + lane] = sum;
@@ -870,17 +905,40 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const mi_attn_args p)
     }
 }
 
+// dT[b][head] = the sum of the blocks' partial sums, in the tiles' order within each of WAVES strides.  Run by blocks of the dK / dV
+// launch behind its tiles (attn_dq_kernel has ended by then): blocks dtable_x of the grid's x, a head each and on.
+template <int WAVES>
+__device__ __forceinline__ bool at_dtable(const mi_attn_args& p)
+{
+    if ((int)(blockIdx.x >> 3) < p.dtable_x) return false;
+    __shared__ float red[WAVES][64];
+    const int b = threadIdx.x & 63, s = threadIdx.x >> 6;
+    for (int head = (blockIdx.x & 7) * p.units_per_xcd + blockIdx.y; head < p.heads; head += 8 * p.units_per_xcd) {
+        float sum = 0.0f;
+        for (int t = s; t < p.dq_tiles; t += WAVES) sum += p.partial[((int64_t)head * p.dq_tiles + t) * MI_ATTN_MAX_BUCKETS + b];
+        red[s][b] = sum;
+        __syncthreads();
+        if (s == 0 && b < p.buckets) {
+            for (int i = 1; i < WAVES; ++i) sum += red[i][b];
+            p.dtable[(int64_t)b * p.heads + head] = sum;
+        }
+        __syncthreads();
+    }
+    return true;
+}
+
 // dK, dV: one block per (key head, share of its query heads, 128 keys), a wave per 32 keys, over the tiles of 64 query rows of
 // the share's heads: S = Q K^T and dP = dO V^T with the key on the lane, dV^T += dO^T P, dK^T += Q^T dS.  Where one block per key
 // head and tile would leave CUs idle the group's heads are shared out over `splits` blocks, whose fp32 sums attn_join_kernel
 // adds in the heads' order.
-template <int DP, bool F16, bool BIAS>
+template <int DP, bool F16, bool BIAS, int KS>
 __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const mi_attn_args p)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    constexpr int BM = 128, TB = AtTile<DP>::BYTES, NB = AT_BUFFERS(DP), PER = 2 * AtStage<DP, 4>::NI + 1;
+    constexpr int BM = 128 / KS, TB = AtTile<DP>::BYTES, NB = AT_BUFFERS(DP), PER = 2 * AtStage<DP, 4>::NI + 1;
     float* const rowv = reinterpret_cast<float*>(lds + NB * 2 * TB);   // [NB][lse in log2 units | D][64]
     float* const vec = rowv + NB * 128;
+    if (BIAS && at_dtable<4>(p)) return;
     int kvh, t, start, len, tile;
     bool tail;
     if (!at_work(p, kvh, t) || !at_find<BM>(p, t, start, len, tile, tail)) return;
@@ -898,7 +956,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const mi_attn_args p)
     if (tile * BM >= len) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
-    const int kw = tile * BM + wave * 32, key = kw + col;
+    // with KS = 2 two waves share 32 keys and take every other 32 rows
+    const int kw = tile * BM + (KS == 1 ? wave : wave & 1) * 32, key = kw + col, s0 = KS == 1 ? 0 : wave >> 1;
     const int64_t ktok = start + (key < len ? key : len - 1);
     u32x4 kf[DP / 16], vf[DP / 16];
     at_load_rows<DP>(kf, p.k, ktok, kvh, p.hd, half);
@@ -957,7 +1016,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const mi_attn_args p)
         const float add = AtPScale<F16>::log2 + (BIAS && !near ? vec[rhi <= -p.reach ? 0 : 2 * R] * p.scale_log2 : 0.0f);
         const int at = key - q0 - 4 * half + R;
 #pragma unroll
-        for (int st = 0; st < 2; ++st) {
+        for (int st = s0; st < (KS == 1 ? 2 : s0 + 1); ++st) {
             if ((q0 + 32 * st >= len || (p.causal && q0 + 32 * st + 31 < kw))) continue;
             f32x16 S = at_first<F16>(near, vec + at - 32 * st, -1, at_rows<DP>(Qt, st, 0, col, half), kf[0]), dP = at_zero16();
 #pragma unroll
@@ -1002,6 +1061,28 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const mi_attn_args p)
             }
         }
     }
+    if constexpr (KS == 2) {
+        at_sync();
+        float* const x = reinterpret_cast<float*>(lds) + (wave & 1) * DP * 64 + lane;
+        if (wave >= 2) {
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    x[(32 * dt + i) * 64] = dK[dt][i];
+                    x[(32 * dt + 16 + i) * 64] = dV[dt][i];
+                }
+        }
+        at_sync();
+        if (wave >= 2) return;
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                dK[dt][i] += x[(32 * dt + i) * 64];
+                dV[dt][i] += x[(32 * dt + 16 + i) * 64];
+            }
+    }
     if (key < len) {
         if (!on) {                                                     // a masked key (the products above ran on its column alone)
 #pragma unroll
@@ -1030,6 +1111,7 @@ __global__ __launch_bounds__(512, 2) void attn_dkv_pair_kernel(const mi_attn_arg
     float* const rowv = reinterpret_cast<float*>(lds + NB * 2 * TB);   // [NB][lse in log2 units | D][64]
     float4* const pass = reinterpret_cast<float4*>(rowv + NB * 128);   // [4 pairs][8][64 lanes]
     float* const vec = reinterpret_cast<float*>(pass + 4 * 8 * 64);
+    if (BIAS && at_dtable<8>(p)) return;
     int kvh, t, start, len, tile;
     bool tail;
     if (!at_work(p, kvh, t) || !at_find<BM>(p, t, start, len, tile, tail)) return;
@@ -1211,21 +1293,6 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const mi_attn_args p)
     *reinterpret_cast<u32x4*>(x.p + token * x.ts + (row % kvh) * x.hs + (i % per) * 8) = o;
 }
 
-// dT[b][head] = the sum of the blocks' partial sums, in the tiles' order within each of 16 strides
-__global__ __launch_bounds__(1024) void attn_dtable_kernel(const mi_attn_args p)
-{
-    __shared__ float red[16][64];
-    const int b = threadIdx.x & 63, s = threadIdx.x >> 6, head = blockIdx.x;
-    float sum = 0.0f;
-    for (int t = s; t < p.tiles; t += 16) sum += p.partial[((int64_t)head * p.tiles + t) * MI_ATTN_MAX_BUCKETS + b];
-    red[s][b] = sum;
-    __syncthreads();
-    if (s == 0 && b < p.buckets) {
-        for (int i = 1; i < 16; ++i) sum += red[i][b];
-        p.dtable[(int64_t)b * p.heads + head] = sum;
-    }
-}
-
 // ---------------------------------------------------------------- launch
 static int gcd_int(int a, int b) { while (b) { const int t = a % b; a = b; b = t; } return a; }
 
@@ -1257,6 +1324,11 @@ static int at_lds(size_t bytes)
     return MI_OK;
 }
 
+// Two waves to a row where 128-row blocks are fewer than four to a CU.  Forward: 432 blocks (2 causal documents up to 4,099, 8 heads of
+// 64, bias) 76 -> 56 us, 520 (8,191, 8 heads of 128) 178 -> 160 us; 1,500 blocks (prompts up to 2,039, 32 heads of 128) 92 us
+// either way, 2,048 (16,384, 16 heads of 128) 1,066 -> 1,243 us, 8,900 (chunks up to 256, 12 heads of 32) 67 -> 83 us.
+static bool at_few(const mi_attn_args& a, int heads) { return (int64_t)heads * (a.tokens / 128 + a.nseq) < 1024; }
+
 template <int DP, bool F16, bool BIAS, int KS>
 static int launch_fwd(hipStream_t st, mi_attn_args& a)
 {
@@ -1273,11 +1345,7 @@ static int launch_fwd(hipStream_t st, mi_attn_args& a)
 template <int DP, bool F16>
 static int launch_fwd(hipStream_t st, mi_attn_args& a)
 {
-    // Two waves to a query where 128-row blocks are fewer than four to a CU: 432 blocks (2 causal documents up to 4,099, 8 heads of
-    // 64, bias) 76 -> 56 us, 520 (8,191, 8 heads of 128) 178 -> 160 us; 1,500 blocks (prompts up to 2,039, 32 heads of 128) 92 us
-    // either way, 2,048 (16,384, 16 heads of 128) 1,066 -> 1,243 us, 8,900 (chunks up to 256, 12 heads of 32) 67 -> 83 us.
-    const int64_t blocks = (int64_t)a.heads * (a.tokens / 128 + a.nseq);
-    const bool split = blocks < 1024;
+    const bool split = at_few(a, a.heads);
     if (a.table) return split ? launch_fwd<DP, F16, true, 2>(st, a) : launch_fwd<DP, F16, true, 1>(st, a);
     return split ? launch_fwd<DP, F16, false, 2>(st, a) : launch_fwd<DP, F16, false, 1>(st, a);
 }
@@ -1307,30 +1375,30 @@ size_t mi_attn_backward_bytes(const mi_attn_args& a)
     const size_t delta = mi_round_up((int64_t)a.heads * a.tokens * 8, 256);
     const int splits = at_dkv_splits(a);
     const size_t join = splits > 1 ? (size_t)mi_round_up((int64_t)splits * 2 * a.tokens * (a.heads / a.group) * a.hd * 4, 256) : 0;
-    const int64_t tiles = a.offsets ? a.tokens / 128 + a.nseq + 1 : (int64_t)a.nseq * ((a.uniform_len + 127) / 128);
+    const int64_t tiles = a.offsets ? a.tokens / 64 + a.nseq + 1 : (int64_t)a.nseq * ((a.uniform_len + 63) / 64);   // at most
     return delta + join + (a.table ? (size_t)(a.heads * tiles) * MI_ATTN_MAX_BUCKETS * 4 : 0);
 }
 
-template <int DP, bool F16, bool BIAS>
+template <int DP, bool F16, bool BIAS, int KS>
 static int launch_dq(hipStream_t st, mi_attn_args& a)
 {
-    const dim3 grid = at_schedule(&a, a.heads, 128);
+    const dim3 grid = at_schedule(&a, a.heads, 128 / KS);
     if (grid.x == 0) return MI_OK;
     const size_t smem = AT_DQ_BUFFERS(DP, BIAS) * 2 * AtTile<DP>::BYTES + (BIAS ? (4 * 32 * 64 + 5 * (2 * (size_t)(a.reach + AT_PAD) + 1)) * 4 : 0);
-    MI_TRY((at_lds<&attn_dq_kernel<DP, F16, BIAS>>(smem)));
-    attn_dq_kernel<DP, F16, BIAS><<<grid, 256, smem, st>>>(a);
+    MI_TRY((at_lds<&attn_dq_kernel<DP, F16, BIAS, KS>>(smem)));
+    attn_dq_kernel<DP, F16, BIAS, KS><<<grid, 256, smem, st>>>(a);
     MI_HIP(hipGetLastError());
     return MI_OK;
 }
 
-template <int DP, bool F16, bool BIAS>
+template <int DP, bool F16, bool BIAS, int KS>
 static int launch_delta(hipStream_t st, mi_attn_args& a)
 {
-    const dim3 grid = at_schedule(&a, a.heads, 128);
+    const dim3 grid = at_schedule(&a, a.heads, 128 / KS);
     if (grid.x == 0) return MI_OK;
     const size_t smem = AT_BUFFERS(DP) * 2 * AtTile<DP>::BYTES + (BIAS ? (size_t)(2 * (a.reach + AT_PAD) + 1) * 4 : 0);
-    MI_TRY((at_lds<&attn_delta_kernel<DP, F16, BIAS>>(smem)));
-    attn_delta_kernel<DP, F16, BIAS><<<grid, 256, smem, st>>>(a);
+    MI_TRY((at_lds<&attn_delta_kernel<DP, F16, BIAS, KS>>(smem)));
+    attn_delta_kernel<DP, F16, BIAS, KS><<<grid, 256, smem, st>>>(a);
     MI_HIP(hipGetLastError());
     return MI_OK;
 }
@@ -1338,15 +1406,17 @@ static int launch_delta(hipStream_t st, mi_attn_args& a)
 template <int DP, bool F16>
 static int launch_bwd(hipStream_t st, mi_attn_args& a)
 {
-    if (a.table) MI_TRY((launch_delta<DP, F16, true>(st, a)));
-    else MI_TRY((launch_delta<DP, F16, false>(st, a)));
-    if (a.table) MI_TRY((launch_dq<DP, F16, true>(st, a)));
-    else MI_TRY((launch_dq<DP, F16, false>(st, a)));
-    if (a.table) {
-        attn_dtable_kernel<<<(unsigned)a.heads, 1024, 0, st>>>(a);
-        MI_HIP(hipGetLastError());
-    }
-    const dim3 grid = at_schedule(&a, a.heads / a.group * a.splits, 128);
+    const bool split = at_few(a, a.heads);
+    if (a.table) MI_TRY((split ? launch_delta<DP, F16, true, 2>(st, a) : launch_delta<DP, F16, true, 1>(st, a)));
+    else MI_TRY((split ? launch_delta<DP, F16, false, 2>(st, a) : launch_delta<DP, F16, false, 1>(st, a)));
+    if (a.table) MI_TRY((split ? launch_dq<DP, F16, true, 2>(st, a) : launch_dq<DP, F16, true, 1>(st, a)));
+    else MI_TRY((split ? launch_dq<DP, F16, false, 2>(st, a) : launch_dq<DP, F16, false, 1>(st, a)));
+    a.dq_tiles = a.tiles;
+    const int units = a.heads / a.group * a.splits;
+    const bool split_kv = DP < 128 && at_few(a, units);
+    dim3 grid = at_schedule(&a, units, split_kv ? 64 : 128);
+    a.dtable_x = (int)(grid.x / 8);
+    if (a.table) grid.x += 8;                                          // the blocks of at_dtable
     if (grid.x == 0) return MI_OK;
     const size_t bias = a.table ? (size_t)(2 * (a.reach + AT_PAD) + 1) * 4 : 0;
     if constexpr (DP == 128) {
@@ -1361,11 +1431,13 @@ static int launch_bwd(hipStream_t st, mi_attn_args& a)
     } else {
         const size_t smem = AT_BUFFERS(DP) * (2 * AtTile<DP>::BYTES + 512) + bias;
         if (a.table) {
-            MI_TRY((at_lds<&attn_dkv_kernel<DP, F16, true>>(smem)));
-            attn_dkv_kernel<DP, F16, true><<<grid, 256, smem, st>>>(a);
+            MI_TRY((at_lds<&attn_dkv_kernel<DP, F16, true, 1>>(smem)));
+            MI_TRY((at_lds<&attn_dkv_kernel<DP, F16, true, 2>>(smem)));
+            if (split_kv) attn_dkv_kernel<DP, F16, true, 2><<<grid, 256, smem, st>>>(a);
+            else attn_dkv_kernel<DP, F16, true, 1><<<grid, 256, smem, st>>>(a);
         } else {
-            MI_TRY((at_lds<&attn_dkv_kernel<DP, F16, false>>(smem)));
-            attn_dkv_kernel<DP, F16, false><<<grid, 256, smem, st>>>(a);
+            if (split_kv) attn_dkv_kernel<DP, F16, false, 2><<<grid, 256, smem, st>>>(a);
+            else attn_dkv_kernel<DP, F16, false, 1><<<grid, 256, smem, st>>>(a);
         }
     }
     MI_HIP(hipGetLastError());
