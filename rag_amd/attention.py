@@ -124,15 +124,69 @@ def packed_attention(q, k, v, offsets=None, *, causal: bool = False, scale: Opti
     both directions (default: not causal).  Rows that attend nothing, and rows behind the last sequence, are 0.
 
     return_lse: also the float32 [heads][tokens] log-sum-exp of each row's scores, which packed_attention_backward takes.  Runs on
-    the current stream of q's device."""
+    the current stream of q's device.
+
+    Differentiable once in q, k, v and bias_table under torch.autograd (out; lse is not).  A step that is captured into a graph
+    calls packed_attention_backward itself: a captured backward pass of autograd may wait for streams outside the capture."""
+    if (q.requires_grad or k.requires_grad or v.requires_grad or (bias_table is not None and bias_table.requires_grad)) and _grad_enabled():
+        out, lse = _function().apply(q, k, v, bias_table, offsets, key_mask, causal, scale, max_distance, bidirectional)
+    else:
+        out, lse = _forward(q, k, v, offsets, causal, scale, key_mask, bias_table, max_distance, bidirectional, return_lse)
+    return (out, lse) if return_lse else out
+
+
+def _forward(q, k, v, offsets, causal, scale, key_mask, bias_table, max_distance, bidirectional, with_lse):
     cfg, tokens, nseq, off, mask, table = _setup(q, k, v, offsets, causal, scale, key_mask, bias_table, max_distance, bidirectional)
     z, dtype, device = q.shape, q.dtype, q.device
     out = q.new_empty(z)
-    lse = q.new_empty((z[-2], tokens), dtype=_F32) if return_lse else None
+    lse = q.new_empty((z[-2], tokens), dtype=_F32) if with_lse else None
     _capi.check(_capi.load().mi_attention_dev(_capi.get_ctx(device.index), cfg, tokens, nseq, off, mask, _rows("q", q, z, dtype, device),
                                               _rows("k", k, k.shape, dtype, device), _rows("v", v, k.shape, dtype, device), table,
-                                              _rows("out", out, z, dtype, device), lse.data_ptr() if return_lse else None, _capi.stream_arg(device)))
-    return (out, lse) if return_lse else out
+                                              _rows("out", out, z, dtype, device), lse.data_ptr() if with_lse else None, _capi.stream_arg(device)))
+    return out, lse
+
+
+def _grad_enabled() -> bool:
+    import torch
+    return torch.is_grad_enabled()
+
+
+def _not_captured(device) -> None:
+    import torch
+    with torch.cuda.device(device):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("packed_attention: autograd under graph capture; call packed_attention(..., return_lse=True) on detached "
+                               "tensors and packed_attention_backward")
+
+
+@functools.lru_cache(maxsize=1)
+def _function():
+    """The autograd node (made on first use: importing this module does not import torch)."""
+    import torch
+    from torch.autograd.function import once_differentiable
+
+    class PackedAttention(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, q, k, v, bias_table, offsets, key_mask, causal, scale, max_distance, bidirectional):
+            if q.is_cuda:
+                _not_captured(q.device)
+            out, lse = _forward(q, k, v, offsets, causal, scale, key_mask, bias_table, max_distance, bidirectional, True)
+            ctx.save_for_backward(q, k, v, bias_table, offsets, key_mask, out, lse)
+            ctx.form = {"causal": causal, "scale": scale, "max_distance": max_distance, "bidirectional": bidirectional}
+            ctx.mark_non_differentiable(lse)
+            return out, lse
+
+        @staticmethod
+        @once_differentiable
+        def backward(ctx, dout, _):
+            q, k, v, bias_table, offsets, key_mask, out, lse = ctx.saved_tensors
+            _not_captured(q.device)
+            if not dout.is_contiguous() or dout.data_ptr() % 16:       # autograd hands over expanded scalars, too
+                dout = dout.clone(memory_format=torch.contiguous_format)
+            grads = packed_attention_backward(dout, q, k, v, out, lse, offsets, key_mask=key_mask, bias_table=bias_table, **ctx.form)
+            return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad)) + (None,) * 6
+
+    return PackedAttention
 
 
 def packed_attention_backward(dout, q, k, v, out, lse, offsets=None, *, causal: bool = False, scale: Optional[float] = None, key_mask=None,
