@@ -362,6 +362,14 @@ int  mi_attention_backward_dev(mi_ctx* ctx, const mi_attention_config* cfg, int6
                                const mi_attention_rows* dq, const mi_attention_rows* dk, const mi_attention_rows* dv,
                                float* dbias_table_dev, void* workspace_dev, size_t workspace_bytes, void* stream);
 
+/* Attention of an encoder's layers: causal, and / or with a relative position bias (bias_table host fp32 [num_buckets][heads],
+ * copied; NULL and num_buckets = 0: none), as mi_attention_dev computes it; causal = 0 without a bias (the state after
+ * mi_encoder_create): the built-in attention.  All layers share the table.  Every entry point of the encoder then computes that model, on
+ * the general kernels at every size.  Waits for the encoder's passes; a pass captured into a graph keeps the form it was
+ * captured with and must not run meanwhile. */
+int  mi_encoder_set_attention(mi_encoder* enc, int causal, const float* bias_table, int num_buckets, int max_distance,
+                              int bidirectional);
+
 /* ---- host text path: WordPiece tokenizer (pure host code, no GPU call)
  * Replaces the tokenizer advanced_rag.py:104-107 reaches through HuggingFaceEmbeddings ->
  * sentence-transformers -> `tokenizers` (BertNormalizer, BertPreTokenizer, WordPiece, [CLS] .. [SEP], truncation):

@@ -35,6 +35,7 @@
 #include <new>
 #include <vector>
 #include "kernels.h"
+#include "attention.h"
 #include "encoder_ffn3.h"
 #include "encoder_qkv_attn.h"
 
@@ -1768,6 +1769,11 @@ struct mi_encoder {
     // cross-encoder head (mi_encoder_set_head): pooler W[H][H] b[H], classifier W[nl][H] b[nl], fp32 on device
     float* head = nullptr;
     int nlabels = 0;
+    // mi_encoder_set_attention: causal or biased attention instead of the built-in one.  The table (device fp32 [buckets][heads],
+    // room for the most buckets) is allocated once, so its address outlives a change of the bias.
+    bool packed_attn = false;
+    mi_attn_args attn;
+    float* bias_table = nullptr;
     // counters since creation: sequences, padded tokens, passes on the bulk / on the latency kernel family
     int64_t st_seqs = 0, st_tokens = 0, st_bulk = 0, st_latency = 0;
     // this device's address of the file-scope `scratch` array (mi_encoder_encode_dev_noalloc)
@@ -1788,6 +1794,7 @@ static void encoder_free(mi_encoder* e)
     if (!e) return;
     for (LayerW& lw : e->layers) { if (lw.bqkv) (void)hipFree(lw.bqkv); if (lw.w3) (void)hipFree(lw.w3); if (lw.p3) (void)hipFree(lw.p3); }
     if (e->blob) (void)hipFree(e->blob);
+    if (e->bias_table) (void)hipFree(e->bias_table);
     if (e->wbf) (void)hipFree(e->wbf);
     for (auto& n : e->ln) {
         if (n.ws) (void)hipFree(n.ws);
@@ -1927,6 +1934,36 @@ extern "C" int mi_encoder_set_head(mi_encoder* e, const float* pooler_w, const f
     MI_HIP(hipMemcpyAsync(d, cls_b, (size_t)num_labels * 4, hipMemcpyHostToDevice, e->stream));
     MI_HIP(hipStreamSynchronize(e->stream));
     e->nlabels = num_labels;
+    return MI_OK;
+}
+
+// Causal attention, and / or a relative position bias (host fp32 [num_buckets][heads]); causal = 0 and num_buckets = 0: the built-in attention.
+extern "C" int mi_encoder_set_attention(mi_encoder* e, int causal, const float* bias_table, int num_buckets, int max_distance, int bidirectional)
+{
+    MI_REQUIRE(e, "mi_encoder_set_attention: NULL argument");
+    MI_REQUIRE((num_buckets == 0) == (bias_table == nullptr), "mi_encoder_set_attention: bias_table goes with num_buckets (%d)", num_buckets);
+    mi_attn_args a;
+    if (num_buckets) MI_TRY(mi_attn_buckets("mi_encoder_set_attention", &a, num_buckets, max_distance, bidirectional));
+    std::lock_guard<std::mutex> lk(e->mu);
+    DeviceGuard guard(e->device);
+    const int NH = e->cfg.num_attention_heads;
+    for (auto& n : e->ln) if (n.have_last) MI_HIP(hipEventSynchronize(n.ev1));   // passes that read the old table
+    if (num_buckets) {
+        if (!e->bias_table) MI_HIP(hipMalloc((void**)&e->bias_table, (size_t)MI_ATTN_MAX_BUCKETS * NH * sizeof(float)));
+        MI_HIP(hipMemcpyAsync(e->bias_table, bias_table, (size_t)num_buckets * NH * sizeof(float), hipMemcpyHostToDevice, e->stream));
+        MI_HIP(hipStreamSynchronize(e->stream));
+        a.table = e->bias_table;
+    }
+    const int64_t H = e->cfg.hidden_size;
+    a.heads = NH;
+    a.hd = (int)(H / NH);
+    a.causal = causal != 0;
+    a.scale_log2 = 1.0f;                             // the Q weights carry head_dim^-0.5 * log2(e)
+    a.q.ts = a.k.ts = a.v.ts = 3 * H;
+    a.out.ts = H;
+    a.q.hs = a.k.hs = a.v.hs = a.out.hs = a.hd;
+    e->attn = a;
+    e->packed_attn = causal || num_buckets;
     return MI_OK;
 }
 
@@ -2142,7 +2179,8 @@ static int encode_pass_locked(mi_encoder* e, int64_t B, int L, const int32_t* id
     const unsigned tok_grid = (unsigned)((T + 3) / 4);
     const int Lp = (L + 31) / 32 * 32;
     const size_t attn_smem = (size_t)Lp * 128 + (size_t)Lp * 4;      // K rows, V rows, additive mask
-    if (attn_smem > 96 * 1024) { mi_set_error("encode: sequence length %d too long for the attention kernel", L); return MI_ERR_UNSUPPORTED; }
+    const bool packed_attn = e->packed_attn;
+    if (!packed_attn && attn_smem > 96 * 1024) { mi_set_error("encode: sequence length %d too long for the attention kernel", L); return MI_ERR_UNSUPPORTED; }
 
     // hidden size 384: the two N = 384 projections run fused with their LayerNorm (MI_GEMM_LN=0: separate kernels)
     static const bool ln_off = getenv("MI_GEMM_LN") && atoi(getenv("MI_GEMM_LN")) == 0;
@@ -2154,7 +2192,8 @@ static int encode_pass_locked(mi_encoder* e, int64_t B, int L, const int32_t* id
     // hand-over (0: always the bulk kernels); read per call so a test can flip it.
     int64_t latency_tokens = 12288;
     if (const char* s = getenv("MI_ENC_LATENCY_TOKENS")) latency_tokens = atoll(s);
-    const bool bulk = T >= latency_tokens;
+    // Causal or biased attention writes row-major context: such a model runs the general GEMMs at every size.
+    const bool bulk = !packed_attn && T >= latency_tokens;
     const bool fused_ln = !ln_off && bulk && H == LN_N && I % 64 == 0;
     static const bool ffn_off = getenv("MI_FFN_FUSED") && atoi(getenv("MI_FFN_FUSED")) == 0;
     const bool fused_ffn = fused_ln && !ffn_off && I == 1536;
@@ -2173,9 +2212,24 @@ static int encode_pass_locked(mi_encoder* e, int64_t B, int L, const int32_t* id
     if (const char* s = getenv("MI_QKV_FUSED_MIN_MEAN")) fused_min_mean = atoll(s);
     const bool qkv_fused = bulk && L <= MI_QKV_ATTN_MAX_L && B <= 65535 && T >= B * fused_min_mean &&
                            !(getenv("MI_QKV_FUSED") && atoi(getenv("MI_QKV_FUSED")) == 0);
+    mi_attn_args attn = e->attn;
+    if (packed_attn) {
+        attn.q.p = qkv;
+        attn.k.p = qkv + H;
+        attn.v.p = qkv + 2 * H;
+        attn.out.p = ctx;
+        attn.offsets = seq_start;
+        attn.key_mask = seq_start ? nullptr : mask;
+        attn.tokens = T;
+        attn.nseq = (int)B;
+        attn.uniform_len = seq_start ? 0 : L;
+    }
     for (const LayerW& lw : e->layers) {
         if (qkv_fused) {
             MI_TRY(mi_launch_qkv_attn(st, h, lw.Wqkv_p, lw.bqkv, mask, seq_start, ctx, B, L, H, NH, fused_ln ? 1 : 0));
+        } else if (packed_attn) {
+            launch_gemm<EPI_BIAS>(st, h, lw.Wqkv, lw.bqkv, nullptr, qkv, (int)T, 3 * H, H, false);
+            MI_TRY(mi_launch_attention(st, attn, MI_DTYPE_BF16));
         } else {
             const bool qkv_blocked = launch_gemm<EPI_BIAS>(st, h, lw.Wqkv, lw.bqkv, nullptr, qkv, (int)T, 3 * H, H, true);
             attn_kernel<<<dim3(NH, (unsigned)B, (L + 255) / 256), 256, attn_smem, st>>>(qkv, mask, seq_start, ctx, L, Lp, H, qkv_blocked ? 1 : 0, fused_ln ? 1 : 0);

@@ -17,7 +17,7 @@ from typing import Any, Dict, List, Optional
 import numpy as np
 
 from . import _capi
-from .encoder_weights import load_local_dir
+from .encoder_weights import load_local_dir, load_local_position_bias
 
 
 class Encoder:
@@ -98,6 +98,21 @@ class Encoder:
                                                        offsets.ctypes.data_as(ctypes.c_void_p), int(max_len), int(max_batch),
                                                        out.ctypes.data_as(ctypes.c_void_p)))
         return out
+
+    def set_attention(self, causal: bool = False, bias_table=None, max_distance: int = 128, bidirectional: Optional[bool] = None) -> None:
+        """Attention of the layers: causal, and / or with a relative position bias learned by buckets (bias_table [num_buckets][heads],
+        shared by the layers; bidirectional: buckets for both directions, default: not causal), as packed_attention computes it.
+        Without arguments: the built-in attention again."""
+        table, buckets = None, 0
+        if bias_table is not None:
+            table = np.ascontiguousarray(bias_table, dtype=np.float32)
+            if table.ndim != 2 or table.shape[0] == 0 or table.shape[1] != self.cfg.num_attention_heads:
+                raise ValueError(f"bias_table must be [num_buckets][{self.cfg.num_attention_heads}], got {table.shape}")
+            buckets = table.shape[0]
+        if bidirectional is None:
+            bidirectional = not causal
+        _capi.check(self._lib.mi_encoder_set_attention(self._h, int(bool(causal)), table.ctypes.data_as(ctypes.c_void_p) if buckets else None,
+                                                       buckets, int(max_distance), int(bool(bidirectional))))
 
     def set_head(self, pooler_w, pooler_b, cls_w, cls_b) -> None:
         """Loads a BertForSequenceClassification head (pooler dense + classifier), fp32."""
@@ -442,7 +457,8 @@ class MI355Embeddings:
     Extensions (none changes a result): `devices=[0, ..., 7]` (or model_kwargs={"devices": [...]}) keeps one encoder per
     listed GPU in this one process and splits every bulk call over them -- pure data parallel, no collective, input
     order kept (BASELINE config 3 from the single process advanced_rag.py is); `slab_texts` is the number of texts
-    tokenised per step of the host pipeline below."""
+    tokenised per step of the host pipeline below.  A model whose directory holds a relative position bias
+    (load_local_position_bias) runs with it; model_kwargs={"causal": True} runs a model trained with causal attention."""
 
     def __init__(self, model_name: str, cache_folder: Optional[str] = None,
                  model_kwargs: Optional[Dict[str, Any]] = None, encode_kwargs: Optional[Dict[str, Any]] = None,
@@ -472,6 +488,11 @@ class MI355Embeddings:
             except (ValueError, _capi.MI355Error):
                 self.native_tokenizer = None
         self.encoders = [Encoder(cfg, blob, device=d) for d in self.devices]
+        bias = load_local_position_bias(model_name)
+        causal = bool(self.model_kwargs.get("causal", False))
+        if causal or bias:
+            for enc in self.encoders:
+                enc.set_attention(causal=causal, **(bias or {}))
         self.encoder = self.encoders[0]
         self.slab_texts = max(1, int(slab_texts))
         self.last_timing: Dict[str, float] = {}

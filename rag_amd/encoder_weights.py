@@ -122,6 +122,44 @@ def random_head(cfg: BertConfig, num_labels: int = 1, seed: int = 0, init_range:
             (rng.standard_normal(num_labels) * init_range).astype(np.float32))
 
 
+def position_bias_from_state_dict(sd: Mapping[str, "np.ndarray"], cfg: Mapping):
+    """Encoder.set_attention's bias arguments, or None: the table encoder.relative_attention_bias.weight [buckets][heads] of a
+    config.json with relative_attention_num_buckets (relative_attention_max_distance: default 128), as relative-position encoders
+    name them.  One table for all layers, buckets for both directions."""
+    buckets = cfg.get("relative_attention_num_buckets")
+    if buckets is None:
+        return None
+    g = {_strip(k): v for k, v in sd.items()}
+    name = "encoder.relative_attention_bias.weight"
+    if name not in g:
+        raise ValueError(f"config.json has relative_attention_num_buckets, but the weights hold no {name}")
+    t = g[name]
+    a = t.detach().cpu().float().numpy() if hasattr(t, "detach") else np.asarray(t, dtype=np.float32)
+    want = (int(buckets), int(cfg["num_attention_heads"]))
+    if tuple(a.shape) != want:
+        raise ValueError(f"{name}: expected shape {want}, got {tuple(a.shape)}")
+    return {"bias_table": np.ascontiguousarray(a, dtype=np.float32), "max_distance": int(cfg.get("relative_attention_max_distance", 128)),
+            "bidirectional": True}
+
+
+def load_local_position_bias(path: str):
+    """position_bias_from_state_dict of a LOCAL directory; None (the weights are not read) for a model without such a bias."""
+    with open(os.path.join(path, "config.json")) as f:
+        cfg = json.load(f)
+    if cfg.get("relative_attention_num_buckets") is None:
+        return None
+    return position_bias_from_state_dict(_load_weights(path), cfg)
+
+
+def _load_weights(path: str):
+    from safetensors.numpy import load_file
+    st = os.path.join(path, "model.safetensors")
+    if not os.path.exists(st):
+        sub = os.path.join(path, "0_Transformer", "model.safetensors")
+        st = sub if os.path.exists(sub) else st
+    return load_file(st)
+
+
 def load_local_dir(path: str, normalize: bool = True, with_head: bool = False):
     """(BertConfig, blob) from a LOCAL directory holding config.json + model.safetensors
     (never a hub name: there is no network on the target machines)."""
@@ -130,12 +168,7 @@ def load_local_dir(path: str, normalize: bool = True, with_head: bool = False):
             f"model_name must be a local directory with config.json and model.safetensors, got {path!r}")
     with open(os.path.join(path, "config.json")) as f:
         cfg = config_from_dict(json.load(f), normalize=normalize)
-    from safetensors.numpy import load_file
-    st = os.path.join(path, "model.safetensors")
-    if not os.path.exists(st):
-        sub = os.path.join(path, "0_Transformer", "model.safetensors")
-        st = sub if os.path.exists(sub) else st
-    sd = load_file(st)
+    sd = _load_weights(path)
     if with_head:
         return cfg, pack_state_dict(sd, cfg), head_from_state_dict(sd, cfg)
     return cfg, pack_state_dict(sd, cfg)

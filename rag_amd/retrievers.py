@@ -219,10 +219,13 @@ class CrossEncoderReranker:
                  score_label: Optional[int] = None):
         from .embeddings import Encoder, _load_tokenizer
         if encoder is None:
-            from .encoder_weights import load_local_dir
+            from .encoder_weights import load_local_dir, load_local_position_bias
             cfg, blob, head = load_local_dir(model_name, normalize=False, with_head=True)
             encoder = Encoder(cfg, blob, device=device)
             encoder.set_head(*head)
+            bias = load_local_position_bias(model_name)
+            if bias:
+                encoder.set_attention(**bias)
             max_length = min(max_length, int(cfg.max_position_embeddings))
             tokenizer = _load_tokenizer(model_name, max_length)
         self.encoder, self.tokenizer, self.max_length, self.activation = encoder, tokenizer, int(max_length), activation

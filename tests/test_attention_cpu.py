@@ -195,3 +195,20 @@ def _forward(q, k, v, table, kw):
                     out[start + i, h] = torch.softmax(s, 0) @ torch.stack([v[start + j, g] for j in js])
         start += n
     return out
+
+
+def test_position_bias_of_a_model():
+    from rag_amd.encoder_weights import position_bias_from_state_dict
+    import torch
+    t = np.arange(12, dtype=np.float32).reshape(6, 2)
+    cfg = {"num_attention_heads": 2, "relative_attention_num_buckets": 6}
+    name = "encoder.relative_attention_bias.weight"
+    assert position_bias_from_state_dict({}, {"num_attention_heads": 2}) is None
+    for prefix in ("", "bert.", "0.auto_model."):
+        got = position_bias_from_state_dict({prefix + name: t}, cfg)
+        assert np.array_equal(got["bias_table"], t) and got["max_distance"] == 128 and got["bidirectional"]
+    assert position_bias_from_state_dict({name: torch.from_numpy(t)}, {**cfg, "relative_attention_max_distance": 40})["max_distance"] == 40
+    with pytest.raises(ValueError, match="hold no"):
+        position_bias_from_state_dict({}, cfg)
+    with pytest.raises(ValueError, match="shape"):
+        position_bias_from_state_dict({name: t[:5]}, cfg)
