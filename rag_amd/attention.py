@@ -17,12 +17,13 @@ from . import _capi
 from ._capi import AttentionConfig, AttentionRows
 
 
-_F32 = _I32 = _CODES = None
+_F32 = _I32 = _CODES = _empty_like = None
 
 
 def _types():
-    global _F32, _I32, _CODES
+    global _F32, _I32, _CODES, _empty_like
     import torch
+    _empty_like = torch.empty_like
     _F32, _I32, _CODES = torch.float32, torch.int32, {torch.bfloat16: _capi.DTYPE_BF16, torch.float16: _capi.DTYPE_F16}
     return _CODES
 
@@ -45,6 +46,11 @@ def _rows(name: str, t, shape, dtype, device) -> AttentionRows:
     # the stride of an axis of one entry is never used; what torch reports for it is arbitrary
     return AttentionRows(t.data_ptr(), s[-3] if z[-3] > 1 else (s[0] if len(z) == 4 and z[0] > 1 else z[-2] * z[-1]),
                          s[-2] if z[-2] > 1 else z[-1])
+
+
+def _like(t):
+    """A new contiguous tensor of t's shape (empty_like is the shorter call, but would keep the strides of a permuted tensor)."""
+    return _empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
 
 
 @functools.lru_cache(maxsize=256)
@@ -138,7 +144,7 @@ def packed_attention(q, k, v, offsets=None, *, causal: bool = False, scale: Opti
 def _forward(q, k, v, offsets, causal, scale, key_mask, bias_table, max_distance, bidirectional, with_lse):
     cfg, tokens, nseq, off, mask, table = _setup(q, k, v, offsets, causal, scale, key_mask, bias_table, max_distance, bidirectional)
     z, dtype, device = q.shape, q.dtype, q.device
-    out = q.new_empty(z)
+    out = _like(q)
     lse = q.new_empty((z[-2], tokens), dtype=_F32) if with_lse else None
     _capi.check(_capi.load().mi_attention_dev(_capi.get_ctx(device.index), cfg, tokens, nseq, off, mask, _rows("q", q, z, dtype, device),
                                               _rows("k", k, k.shape, dtype, device), _rows("v", v, k.shape, dtype, device), table,
@@ -202,8 +208,8 @@ def packed_attention_backward(dout, q, k, v, out, lse, offsets=None, *, causal: 
         raise ValueError(f"packed_attention_backward: lse must be the contiguous float32 [{heads}][{tokens}] tensor of the forward pass")
     rows = (_rows("q", q, z, dtype, device), _rows("k", k, zk, dtype, device), _rows("v", v, zk, dtype, device), _rows("out", out, z, dtype, device),
             _rows("dout", dout, z, dtype, device))
-    dq, dk, dv = q.new_empty(z), k.new_empty(zk), v.new_empty(zk)
-    dtable = bias_table.new_empty(bias_table.shape) if bias_table is not None else None
+    dq, dk, dv = _like(q), _like(k), _like(v)
+    dtable = _like(bias_table) if bias_table is not None else None
     work = q.new_empty(_workspace(heads, zk[-2], z[-1], cfg.num_buckets, cfg.max_distance, cfg.bidirectional, tokens, nseq, offsets is not None), dtype=_F32)
     _capi.check(_capi.load().mi_attention_backward_dev(_capi.get_ctx(device.index), cfg, tokens, nseq, off, mask, rows[0], rows[1], rows[2], table, rows[3],
                                               lse.data_ptr(), rows[4], _rows("dq", dq, z, dtype, device), _rows("dk", dk, zk, dtype, device),

@@ -638,112 +638,18 @@ __global__ __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) void attn_fwd
 // thousands of keys has p near fp16's subnormals), and ds = p (dp - D) takes the scale back out.
 template <bool F16> struct AtPScale { static constexpr float log2 = F16 ? 12.0f : 0.0f, up = F16 ? 4096.0f : 1.0f, down = F16 ? 1.0f / 4096.0f : 1.0f; };
 
-// D = sum_j p dp of every row.  rowsum(dout * out) is the same sum, but takes over the rounding of p and out in the forward pass,
-// which shows in rows of few keys (20 causal rows: dq and dk 1.65 x the plain rounding of their values, 1.4 with D exact) and in
-// the table's gradient, a sum of many ds that nearly cancel.  So with a bias, for rows of up to 128 keys, and for up to 512 where
-// a mask may leave few of them, the sum is made from the scores, in fp32; other rows take the dot product.  Also writes the rows'
-// log-sum-exp the way the other two kernels take it: in log2 units, +inf for a row that attends nothing.
-template <int DP, bool F16, bool BIAS, int KS>
-__global__ __launch_bounds__(256, 2) void attn_delta_kernel(const mi_attn_args p)
-{
-    extern __shared__ __attribute__((aligned(16))) char lds[];
-    constexpr int BM = 128 / KS, TB = AtTile<DP>::BYTES, NB = AT_BUFFERS(DP);
-    float* const vec = reinterpret_cast<float*>(lds + NB * 2 * TB);
-    int head, t, start, len, tile;
-    bool tail;
-    if (!at_work(p, head, t) || !at_find<BM>(p, t, start, len, tile, tail) || tail || tile * BM >= len) return;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 31, half = lane >> 5;
-    if (p.causal) tile = (len + BM - 1) / BM - 1 - tile;
-    const int qw = tile * BM + (KS == 1 ? wave : wave & 1) * 32, q = qw + col, s0 = KS == 1 ? 0 : wave >> 1;   // as in attn_fwd_kernel
-    const int kend = p.causal ? (tile * BM + BM < len ? tile * BM + BM : len) : len;
-    const int64_t tok = start + (q < len ? q : len - 1);
-    const bool mask = p.key_mask != nullptr;
-    u32x4 df[DP / 16], qf[DP / 16];                                    // qf: rows of out, or of q
-    at_load_rows<DP>(df, p.dout, tok, head, p.hd, half);
-    float nl = p.lse[(int64_t)head * p.tokens + tok] * AT_LOG2E;
-    if (nl == -INFINITY) nl = INFINITY;                                // a row that attends nothing: p = 0
-    float a = 0.0f, c = 0.0f;
-    if (!BIAS && kend > (mask ? 512 : 128)) {
-        at_load_rows<DP>(qf, p.out, tok, head, p.hd, half);
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                a = __builtin_fmaf(at_lo<F16>(df[s][j]), at_lo<F16>(qf[s][j]), a);
-                a = __builtin_fmaf(at_hi<F16>(df[s][j]), at_hi<F16>(qf[s][j]), a);
-            }
-        c = half == 0 ? 1.0f : 0.0f;
-        if (s0 > 0) a = c = 0.0f;                                      // (the other wave of the row has it)
-    } else {
-        at_load_rows<DP>(qf, p.q, tok, head, p.hd, half);
-        __shared__ uint64_t words[AT_WORDS];
-        AtKeys keys;
-        keys.init(p.key_mask, words, start, len, kend, wave, 4, lane);
-        AtPipe<DP, NB> pipe;
-        pipe.a.init(p.k, start, 0, len, at_div(head, p.group_inv), p.hd, wave, lane);
-        pipe.b.init(p.v, start, 0, len, at_div(head, p.group_inv), p.hd, wave, lane);
-        pipe.start(lds, &keys, wave);
-        if constexpr (BIAS) at_fill_bias(p, head, AT_LOG2E, 0.0f, vec);
-        const int R = p.reach + AT_PAD;
-        for (int k0 = 0; k0 < pipe.n * AT_KT; k0 += AT_KT) {
-            const char* const Kt = lds + pipe.next(k0 / AT_KT);
-            if (qw >= len || (p.causal && k0 + 32 * s0 > qw + 31)) continue;
-            const uint64_t on = keys.tile(k0 / AT_KT);
-            const int rlo = k0 - (qw + 31), rhi = k0 + AT_KT - 1 - qw;
-            const bool near = BIAS && rhi > -p.reach && rlo < p.reach;
-            const float far = BIAS && !near ? vec[rhi <= -p.reach ? 0 : 2 * R] - nl : -nl;
-            const float* const bv = vec + (k0 + 4 * half - q + R);
-#pragma unroll
-            for (int st = s0; st < (KS == 1 ? 2 : s0 + 1); ++st) {
-                if (st > 0 && (k0 + 32 >= kend || (p.causal && k0 + 32 > qw + 31))) break;
-                f32x16 S = at_zero16(), dP = at_zero16();
-#pragma unroll
-                for (int s = 0; s < DP / 16; ++s) S = at_mfma<F16>(at_rows<DP>(Kt, st, s, col, half), qf[s], S);
-#pragma unroll
-                for (int s = 0; s < DP / 16; ++s) dP = at_mfma<F16>(at_rows<DP>(Kt + TB, st, s, col, half), df[s], dP);
-                if (near) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) S[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], p.scale_log2, bv[32 * st + 8 * (i >> 2) + (i & 3)] - nl));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) S[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], p.scale_log2, far));
-                }
-                at_unattended(p, mask, (uint32_t)(on >> (32 * st)), k0 + 32 * st, qw, q, len, half, [&](int i, bool yes) __attribute__((always_inline)) {
-                    S[i] = yes ? S[i] : 0.0f;
-                    dP[i] = yes ? dP[i] : 0.0f;
-                });
-                float a1 = 0.0f, c1 = 0.0f;                            // (short chains: a long row's sums stay exact to fp32's last bits)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) { a1 = __builtin_fmaf(S[i], dP[i], a1); c1 += S[i]; }
-                a += a1;
-                c += c1;
-            }
-        }
-    }
-    a += at_other_half(a);
-    c += at_other_half(c);
-    if constexpr (KS == 2) {
-        at_sync();
-        float* const x = reinterpret_cast<float*>(lds) + (wave & 1) * 128 + lane;
-        if (wave >= 2) {
-            x[0] = a;
-            x[64] = c;
-        }
-        at_sync();
-        if (wave >= 2) return;
-        a += x[0];
-        c += x[64];
-    }
-    if (half == 0 && q < len) {
-        p.delta[(int64_t)head * p.tokens + tok] = c == 0.0f ? a : a / c;
-        p.lse2[(int64_t)head * p.tokens + tok] = nl;
-    }
-}
-
 #define AT_DQ_BUFFERS(DP, BIAS) ((BIAS) ? ((DP) == 32 ? 3 : 2) : AT_BUFFERS(DP))
 // dQ: one block per (head, 128 query rows), like the forward pass: S^T = K Q^T and dP^T = V dO^T with the query on the lane,
-// dQ^T += K^T dS^T.
+// dQ^T += K^T dS^T, with ds = p (dp - D).
+//
+// D = sum_j p dp of a row.  rowsum(dout * out) is the same sum, but takes over the rounding of p and out in the forward pass,
+// which shows in rows of few keys (20 causal rows: dq and dk 1.65 x the plain rounding of their values, 1.4 with D exact) and in
+// the table's gradient, a sum of many ds that nearly cancel.  So with a bias, for rows of up to 128 keys, and for up to 512 where
+// a mask may leave few of them, a first pass over the keys makes the sum from the scores, in fp32 (its tiles are still in LDS for
+// the second where they fit); other rows take the dot product.  D and the rows' log-sum-exp in log2 units, +inf for a row that
+// attends nothing, are left for the dK / dV kernel.  A kernel of its own for D
+// was slower: 8 queries of 5 - 31 tokens (12 heads of 32, bias) 14.3 -> 10.2 us, 96 chunks up to 256 67 -> 59, 24 passages up to 511
+// (12 x 64) 73 -> 65, 9 causal prompts up to 2,048 (16 x 128, no bias) 87 -> 78.
 //
 // BIAS: the table's gradient is the sum of ds along the diagonals r = key - query.  A 32 x 32 block of ds goes through a skewed
 // image in LDS, element (key, query) at [query][key - query + 31], so that lane l finds a diagonal in column l (the positions a row
@@ -775,6 +681,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const mi_attn_args p)
     const int kvh = at_div(head, p.group_inv);
 
     __shared__ uint64_t words[AT_WORDS];
+    __shared__ float pair[4][2][64];
     AtKeys keys;
     keys.init(p.key_mask, words, start, len, kend, wave, 4, lane);
     const bool mask = keys.mask != nullptr;
@@ -787,8 +694,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const mi_attn_args p)
     const int64_t tok = start + (q < len ? q : len - 1);
     at_load_rows<DP>(qf, p.q, tok, head, p.hd, half);
     at_load_rows<DP>(df, p.dout, tok, head, p.hd, half);
-    const float D = p.delta[(int64_t)head * p.tokens + tok];
-    const float nl = q < len ? p.lse2[(int64_t)head * p.tokens + tok] : INFINITY;   // +inf: p = 0
+    float nl = p.lse[(int64_t)head * p.tokens + tok] * AT_LOG2E;
+    if (nl == -INFINITY || q >= len) nl = INFINITY;                    // p = 0
 
     float* const skew = skew0 + wave * 32 * 64;
     float* const dvec = dvec0 + wave * nvec;
@@ -799,60 +706,116 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const mi_attn_args p)
         for (int i = 0; i < 32; ++i) skew[i * 64 + lane] = 0.0f;
         for (int i = lane; i < nvec; i += 64) dvec[i] = 0.0f;
     }
+
+    // calls use(tile, K tile, 32-key block, p, dp, ...) with p = 0 and dp = 0 where a key is not attended
+    auto walk = [&](auto use) __attribute__((always_inline)) {
+        for (int k0 = 0; k0 < pipe.n * AT_KT; k0 += AT_KT) {
+            const char* const Kt = lds + pipe.next(k0 / AT_KT);
+            if (qw >= len || (p.causal && k0 + 32 * s0 > qw + 31)) continue;
+            const uint64_t on = keys.tile(k0 / AT_KT);
+            const int rlo = k0 - (qw + 31), rhi = k0 + AT_KT - 1 - qw;
+            const bool near = BIAS && rhi > -p.reach && rlo < p.reach;
+            const float far = BIAS && !near ? __builtin_fmaf(vec[rhi <= -p.reach ? 0 : 2 * R], p.scale_log2, -nl) : -nl;
+            const float* const bv = vec + (k0 + 4 * half - q + R);
+#pragma unroll
+            for (int st = s0; st < (KS == 1 ? 2 : s0 + 1); ++st) {
+                if (st > 0 && (k0 + 32 >= kend || (p.causal && k0 + 32 > qw + 31))) break;
+                f32x16 S = at_first<F16>(near, bv + 32 * st, 1, at_rows<DP>(Kt, st, 0, col, half), qf[0]), dP = at_zero16();
+#pragma unroll
+                for (int s = 1; s < DP / 16; ++s) S = at_mfma<F16>(at_rows<DP>(Kt, st, s, col, half), qf[s], S);
+#pragma unroll
+                for (int s = 0; s < DP / 16; ++s) dP = at_mfma<F16>(at_rows<DP>(Kt + TB, st, s, col, half), df[s], dP);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) S[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], p.scale_log2, far));
+                at_unattended(p, mask, (uint32_t)(on >> (32 * st)), k0 + 32 * st, qw, q, len, half, [&](int i, bool yes) __attribute__((always_inline)) {
+                    S[i] = yes ? S[i] : 0.0f;
+                    dP[i] = yes ? dP[i] : 0.0f;
+                });
+                use(Kt, st, S, dP, near, rlo, rhi);
+            }
+        }
+    };
+
+    float D = 0.0f, fix = 1.0f;                                        // fix: over the sum of p as it is rebuilt (the saved log-sum-exp is off by up to 5e-7)
+    if (!BIAS && kend > (mask ? 512 : 128)) {
+        u32x4 of[DP / 16];
+        at_load_rows<DP>(of, p.out, tok, head, p.hd, half);
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                D = __builtin_fmaf(at_lo<F16>(df[s][j]), at_lo<F16>(of[s][j]), D);
+                D = __builtin_fmaf(at_hi<F16>(df[s][j]), at_hi<F16>(of[s][j]), D);
+            }
+        D += at_other_half(D);
+    } else {
+        float c = 0.0f;
+        walk([&](const char*, int, const f32x16& S, const f32x16& dP, bool, int, int) __attribute__((always_inline)) {
+            float a1 = 0.0f, c1 = 0.0f;                                // (short chains: a long row's sums stay exact to fp32's last bits)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { a1 = __builtin_fmaf(S[i], dP[i], a1); c1 += S[i]; }
+            D += a1;
+            c += c1;
+        });
+        D += at_other_half(D);
+        c += at_other_half(c);
+        if (KS == 2) {
+            pair[wave][0][lane] = D;
+            pair[wave][1][lane] = c;
+        }
+        at_sync();                                                     // (every wave is done with the tiles)
+        if (KS == 2) {
+            D += pair[wave ^ 2][0][lane];
+            c += pair[wave ^ 2][1][lane];
+        }
+        if (c != 0.0f) fix = 1.0f / c;
+        D *= fix;
+        if (pipe.n < NB) {
+            pipe.buf = NB - 1;                                         // all tiles are where they were
+        } else {
+            pipe.a.init(p.k, start, 0, len, kvh, p.hd, wave, lane);
+            pipe.b.init(p.v, start, 0, len, kvh, p.hd, wave, lane);
+            pipe.start(lds, &keys, wave);
+        }
+    }
+    if (half == 0 && q < len && (KS == 1 || wave < 2)) {
+        p.delta[(int64_t)head * p.tokens + tok] = D;
+        p.lse2[(int64_t)head * p.tokens + tok] = nl;
+    }
+
+    const float Df = D * fix;
     f32x16 dQ[DP / 32];
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) dQ[dt] = at_zero16();
-
-    for (int k0 = 0; k0 < pipe.n * AT_KT; k0 += AT_KT) {
-        const char* const Kt = lds + pipe.next(k0 / AT_KT);
-        if (qw >= len || (p.causal && k0 + 32 * s0 > qw + 31)) continue;
-        const uint64_t on = keys.tile(k0 / AT_KT);
-        const int rlo = k0 - (qw + 31), rhi = k0 + AT_KT - 1 - qw;
-        const bool near = BIAS && rhi > -p.reach && rlo < p.reach;
-        const float far = BIAS && !near ? __builtin_fmaf(vec[rhi <= -p.reach ? 0 : 2 * R], p.scale_log2, -nl) : -nl;
-        const float* const bv = vec + (k0 + 4 * half - q + R);
+    walk([&](const char* Kt, int st, const f32x16& S, f32x16& dP, bool near, int rlo, int rhi) __attribute__((always_inline)) {
 #pragma unroll
-        for (int st = s0; st < (KS == 1 ? 2 : s0 + 1); ++st) {
-            if (st > 0 && (k0 + 32 >= kend || (p.causal && k0 + 32 > qw + 31))) break;
-            f32x16 S = at_first<F16>(near, bv + 32 * st, 1, at_rows<DP>(Kt, st, 0, col, half), qf[0]), dP = at_zero16();
+        for (int i = 0; i < 16; ++i) dP[i] = S[i] * __builtin_fmaf(dP[i], fix, -Df);   // ds
+        if constexpr (BIAS) {
+            if (near) {
+                float* const at = skew + col * 63 + 31 + 4 * half;
 #pragma unroll
-            for (int s = 1; s < DP / 16; ++s) S = at_mfma<F16>(at_rows<DP>(Kt, st, s, col, half), qf[s], S);
+                for (int i = 0; i < 16; ++i) at[8 * (i >> 2) + (i & 3)] = dP[i];
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int s = 0; s < DP / 16; ++s) dP = at_mfma<F16>(at_rows<DP>(Kt + TB, st, s, col, half), df[s], dP);
+                for (int i = 0; i < 32; ++i) sum[i & 3] += skew[i * 64 + lane];
+                if (lane < 63) dvec[rlo + 32 * st + R + lane] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            } else {
+                float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < 16; ++i) S[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], p.scale_log2, far));
-            // ds, over dp
-#pragma unroll
-            for (int i = 0; i < 16; ++i) dP[i] = S[i] * (dP[i] - D);
-            at_unattended(p, mask, (uint32_t)(on >> (32 * st)), k0 + 32 * st, qw, q, len, half,
-                          [&](int i, bool yes) __attribute__((always_inline)) { dP[i] = yes ? dP[i] : 0.0f; });
-            if constexpr (BIAS) {
-                if (near) {
-                    float* const at = skew + col * 63 + 31 + 4 * half;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) at[8 * (i >> 2) + (i & 3)] = dP[i];
-                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) sum[i & 3] += skew[i * 64 + lane];
-                    if (lane < 63) dvec[rlo + 32 * st + R + lane] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                } else {
-                    float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) sum[i & 1] += dP[i];
-                    farS[0] += rhi <= -p.reach ? sum[0] + sum[1] : 0.0f;
-                    farS[1] += rhi <= -p.reach ? 0.0f : sum[0] + sum[1];
-                }
-            }
-#pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                u32x4 sf;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sf[i] = at_pack2<F16>(dP[8 * kk + 2 * i], dP[8 * kk + 2 * i + 1]);
-#pragma unroll
-                for (int dt = 0; dt < DP / 32; ++dt) dQ[dt] = at_mfma<F16>(at_cols<DP>(Kt, 2 * st + kk, dt, lane), sf, dQ[dt]);
+                for (int i = 0; i < 16; ++i) sum[i & 1] += dP[i];
+                farS[0] += rhi <= -p.reach ? sum[0] + sum[1] : 0.0f;
+                farS[1] += rhi <= -p.reach ? 0.0f : sum[0] + sum[1];
             }
         }
-    }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            u32x4 sf;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sf[i] = at_pack2<F16>(dP[8 * kk + 2 * i], dP[8 * kk + 2 * i + 1]);
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; ++dt) dQ[dt] = at_mfma<F16>(at_cols<DP>(Kt, 2 * st + kk, dt, lane), sf, dQ[dt]);
+        }
+    });
     if constexpr (KS == 2) {
         at_sync();
         float* const x = reinterpret_cast<float*>(lds) + (wave & 1) * (DP / 2) * 64 + lane;
@@ -1391,24 +1354,10 @@ static int launch_dq(hipStream_t st, mi_attn_args& a)
     return MI_OK;
 }
 
-template <int DP, bool F16, bool BIAS, int KS>
-static int launch_delta(hipStream_t st, mi_attn_args& a)
-{
-    const dim3 grid = at_schedule(&a, a.heads, 128 / KS);
-    if (grid.x == 0) return MI_OK;
-    const size_t smem = AT_BUFFERS(DP) * 2 * AtTile<DP>::BYTES + (BIAS ? (size_t)(2 * (a.reach + AT_PAD) + 1) * 4 : 0);
-    MI_TRY((at_lds<&attn_delta_kernel<DP, F16, BIAS, KS>>(smem)));
-    attn_delta_kernel<DP, F16, BIAS, KS><<<grid, 256, smem, st>>>(a);
-    MI_HIP(hipGetLastError());
-    return MI_OK;
-}
-
 template <int DP, bool F16>
 static int launch_bwd(hipStream_t st, mi_attn_args& a)
 {
     const bool split = at_few(a, a.heads);
-    if (a.table) MI_TRY((split ? launch_delta<DP, F16, true, 2>(st, a) : launch_delta<DP, F16, true, 1>(st, a)));
-    else MI_TRY((split ? launch_delta<DP, F16, false, 2>(st, a) : launch_delta<DP, F16, false, 1>(st, a)));
     if (a.table) MI_TRY((split ? launch_dq<DP, F16, true, 2>(st, a) : launch_dq<DP, F16, true, 1>(st, a)));
     else MI_TRY((split ? launch_dq<DP, F16, false, 2>(st, a) : launch_dq<DP, F16, false, 1>(st, a)));
     a.dq_tiles = a.tiles;
