@@ -31,13 +31,14 @@ def _types():
 def _rows(name: str, t, shape, dtype, device) -> AttentionRows:
     """A [tokens][heads][head_dim] or [batch][length][heads][head_dim] tensor as mi_attention_rows (views are fine while head_dim is
     adjacent and a batch's rows are evenly spaced)."""
-    z = t.shape
-    if t.dtype != dtype or t.device != device:
+    if t.dtype is not dtype or t.device != device:
         raise ValueError(f"packed_attention: {name} is {t.dtype} on {t.device}, q is {dtype} on {device}")
-    if z != shape:
-        raise ValueError(f"packed_attention: {name} has shape {tuple(z)}, {tuple(shape)} is wanted")
+    if t.shape != shape:
+        raise ValueError(f"packed_attention: {name} has shape {tuple(t.shape)}, {tuple(shape)} is wanted")
+    z = shape
     if t.is_contiguous():
-        return AttentionRows(t.data_ptr(), z[-2] * z[-1], z[-1])
+        hd = z[-1]
+        return AttentionRows(t.data_ptr(), z[-2] * hd, hd)
     s = t.stride()
     if z[-1] > 1 and s[-1] != 1:
         raise ValueError(f"packed_attention: the head_dim elements of {name} must be adjacent (strides {s})")
@@ -46,6 +47,11 @@ def _rows(name: str, t, shape, dtype, device) -> AttentionRows:
     # the stride of an axis of one entry is never used; what torch reports for it is arbitrary
     return AttentionRows(t.data_ptr(), s[-3] if z[-3] > 1 else (s[0] if len(z) == 4 and z[0] > 1 else z[-2] * z[-1]),
                          s[-2] if z[-2] > 1 else z[-1])
+
+
+def _own_rows(t, heads, hd) -> AttentionRows:
+    """... of a contiguous tensor made here: nothing to check."""
+    return AttentionRows(t.data_ptr(), heads * hd, hd)
 
 
 def _like(t):
@@ -143,12 +149,12 @@ def packed_attention(q, k, v, offsets=None, *, causal: bool = False, scale: Opti
 
 def _forward(q, k, v, offsets, causal, scale, key_mask, bias_table, max_distance, bidirectional, with_lse):
     cfg, tokens, nseq, off, mask, table = _setup(q, k, v, offsets, causal, scale, key_mask, bias_table, max_distance, bidirectional)
-    z, dtype, device = q.shape, q.dtype, q.device
+    z, zk, dtype, device = q.shape, k.shape, q.dtype, q.device
     out = _like(q)
     lse = q.new_empty((z[-2], tokens), dtype=_F32) if with_lse else None
     _capi.check(_capi.load().mi_attention_dev(_capi.get_ctx(device.index), cfg, tokens, nseq, off, mask, _rows("q", q, z, dtype, device),
-                                              _rows("k", k, k.shape, dtype, device), _rows("v", v, k.shape, dtype, device), table,
-                                              _rows("out", out, z, dtype, device), lse.data_ptr() if with_lse else None, _capi.stream_arg(device)))
+                                              _rows("k", k, zk, dtype, device), _rows("v", v, zk, dtype, device), table,
+                                              _own_rows(out, z[-2], z[-1]), lse.data_ptr() if with_lse else None, _capi.stream_arg(device)))
     return out, lse
 
 
@@ -212,7 +218,7 @@ def packed_attention_backward(dout, q, k, v, out, lse, offsets=None, *, causal: 
     dtable = _like(bias_table) if bias_table is not None else None
     work = q.new_empty(_workspace(heads, zk[-2], z[-1], cfg.num_buckets, cfg.max_distance, cfg.bidirectional, tokens, nseq, offsets is not None), dtype=_F32)
     _capi.check(_capi.load().mi_attention_backward_dev(_capi.get_ctx(device.index), cfg, tokens, nseq, off, mask, rows[0], rows[1], rows[2], table, rows[3],
-                                              lse.data_ptr(), rows[4], _rows("dq", dq, z, dtype, device), _rows("dk", dk, zk, dtype, device),
-                                              _rows("dv", dv, zk, dtype, device), dtable.data_ptr() if dtable is not None else None, work.data_ptr(),
+                                              lse.data_ptr(), rows[4], _own_rows(dq, heads, z[-1]), _own_rows(dk, zk[-2], z[-1]),
+                                              _own_rows(dv, zk[-2], z[-1]), dtable.data_ptr() if dtable is not None else None, work.data_ptr(),
                                               work.numel() * 4, _capi.stream_arg(device)))
     return dq, dk, dv, dtable

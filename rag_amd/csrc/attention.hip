@@ -444,8 +444,10 @@ __device__ __forceinline__ f32x16 at_first(bool near, const float* bv, int step,
 // ---------------------------------------------------------------- forward
 #define AT_BUFFERS(DP) ((DP) == 32 ? 4 : (DP) == 64 ? 3 : 2)          // what leaves LDS for as many blocks as the registers do
 // One block per (head, 128 / KS query rows): four waves, each 32 queries by every KS-th 32-key block of the K and V tiles, which come by
-// LDS-DMA, 64 keys at a time, one barrier per tile.  With KS = 2 the two
-// waves of a query join their sums through LDS at the end: half the time per tile and twice the blocks, for calls of few blocks.
+// LDS-DMA, 64 keys at a time, one barrier per tile.  With KS = 2 the two waves of a query join their sums through LDS at the end:
+// half the time per tile and twice the blocks, for calls of few blocks.  Bound: head size 128 by the products (16,384 tokens causal, 16
+// heads on 2, 1,064 us, 1,030 TFLOP/s of the 1,127 a large fp16 product reaches), 32 and 64 by the exponentials and what
+// goes with them (400 chunks up to 256 tokens, 12 heads of 32, bias: 70 us; 64 x 512 padded, 12 heads of 64: 67 us).
 template <int DP, bool F16, bool BIAS, int KS>
 __global__ __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) void attn_fwd_kernel(const mi_attn_args p)
 {
@@ -636,7 +638,7 @@ __global__ __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) void attn_fwd
 // ---------------------------------------------------------------- backward
 // P is rebuilt from the saved log-sum-exp.  fp16 only: p is scaled by 2^12 on its way into the 16-bit operand of dV (a row of
 // thousands of keys has p near fp16's subnormals), and ds = p (dp - D) takes the scale back out.
-template <bool F16> struct AtPScale { static constexpr float log2 = F16 ? 12.0f : 0.0f, up = F16 ? 4096.0f : 1.0f, down = F16 ? 1.0f / 4096.0f : 1.0f; };
+template <bool F16> struct AtPScale { static constexpr float log2 = F16 ? 12.0f : 0.0f, down = F16 ? 1.0f / 4096.0f : 1.0f; };
 
 #define AT_DQ_BUFFERS(DP, BIAS) ((BIAS) ? ((DP) == 32 ? 3 : 2) : AT_BUFFERS(DP))
 // dQ: one block per (head, 128 query rows), like the forward pass: S^T = K Q^T and dP^T = V dO^T with the query on the lane,
@@ -654,7 +656,8 @@ template <bool F16> struct AtPScale { static constexpr float log2 = F16 ? 12.0f 
 // BIAS: the table's gradient is the sum of ds along the diagonals r = key - query.  A 32 x 32 block of ds goes through a skewed
 // image in LDS, element (key, query) at [query][key - query + 31], so that lane l finds a diagonal in column l (the positions a row
 // never writes hold the zeros they started with); the 63 sums are added to the wave's vector over r.  A tile of one bucket adds
-// in registers.  Every sum has one owner and a fixed order.  @DQ_BIAS@
+// in registers.  Every sum has one owner and a fixed order.  (LDS float atomics, the direct form, took 122 clocks a wave instruction;
+// diagonals as rows of 36 floats, read 16 bytes a lane, the same time.)
 template <int DP, bool F16, bool BIAS, int KS>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const mi_attn_args p)
 {
@@ -893,7 +896,7 @@ __device__ __forceinline__ bool at_dtable(const mi_attn_args& p)
 // dK, dV: one block per (key head, share of its query heads, 128 keys), a wave per 32 keys, over the tiles of 64 query rows of
 // the share's heads: S = Q K^T and dP = dO V^T with the key on the lane, dV^T += dO^T P, dK^T += Q^T dS.  Where one block per key
 // head and tile would leave CUs idle the group's heads are shared out over `splits` blocks, whose fp32 sums attn_join_kernel
-// adds in the heads' order.
+// adds in the heads' order.  96 chunks up to 256 tokens (12 heads of 32, bias) take 33 us, a document of 4,000 (8 heads of 64) 68.
 template <int DP, bool F16, bool BIAS, int KS>
 __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const mi_attn_args p)
 {
@@ -1062,7 +1065,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const mi_attn_args p)
 }
 
 // The same at head sizes above 64, where dK, dV, K and V of 32 keys (192 registers and what the products need) leave a SIMD one wave,
-// which nothing overlaps with: 1 x 8,191 causal, 8 heads of 128, 412 us where this form takes @PAIR@ us.  Eight waves, two to 32 keys: wave A
+// which nothing overlaps with: 1 x 8,191 causal, 8 heads of 128, 412 us where this form takes 362 us.  Eight waves, two to 32 keys: wave A
 // makes S and P and sums dV, wave B makes dP and dS and sums dK.  P goes from A to B through LDS in fp32, each register to the same
 // lane's; a SIMD has one wave of either kind, so one's exponentials run beside the other's products.  Two barriers a tile: it has
 // landed, P is there.
@@ -1289,7 +1292,8 @@ static int at_lds(size_t bytes)
 
 // Two waves to a row where 128-row blocks are fewer than four to a CU.  Forward: 432 blocks (2 causal documents up to 4,099, 8 heads of
 // 64, bias) 76 -> 56 us, 520 (8,191, 8 heads of 128) 178 -> 160 us; 1,500 blocks (prompts up to 2,039, 32 heads of 128) 92 us
-// either way, 2,048 (16,384, 16 heads of 128) 1,066 -> 1,243 us, 8,900 (chunks up to 256, 12 heads of 32) 67 -> 83 us.
+// either way, 2,048 (16,384, 16 heads of 128) 1,066 -> 1,243 us, 8,900 (chunks up to 256, 12 heads of 32) 67 -> 83 us.  Backward: 256
+// blocks (a document of 4,000, 8 heads of 64, bias) dQ 98 -> 73 us, dK / dV 99 -> 68 us; 512 (8,191, 8 heads of 128) dQ 255 -> 228 us.
 static bool at_few(const mi_attn_args& a, int heads) { return (int64_t)heads * (a.tokens / 128 + a.nseq) < 1024; }
 
 template <int DP, bool F16, bool BIAS, int KS>
@@ -1323,7 +1327,8 @@ int mi_launch_attention(hipStream_t st, mi_attn_args a, int dtype)
 
 // Shares of a group's query heads in the dK / dV kernel: the fewest that give AT_DKV_BLOCKS blocks (two per CU, four rounds, so
 // that a causal sequence's long first tiles even out), all heads at most.  1 x 8,191 causal, 8 heads on 2 key heads of 128:
-// 128 blocks 1,620 us, 512 blocks @DKV_SPLIT@ us.
+// 130 blocks 1,240 us, 520 blocks 362 us and 12 for joining; 9 prompts up to 2,048, 16 heads on 4: 192 blocks 321, 384 blocks 173 + 10,
+// 768 blocks 123 + 15.
 #define AT_DKV_BLOCKS 2048
 static int at_dkv_splits(const mi_attn_args& a)
 {
@@ -1378,10 +1383,8 @@ static int launch_bwd(hipStream_t st, mi_attn_args& a)
             attn_dkv_pair_kernel<F16, false><<<grid, 512, smem, st>>>(a);
         }
     } else {
-        const size_t smem = AT_BUFFERS(DP) * (2 * AtTile<DP>::BYTES + 512) + bias;
+        const size_t smem = AT_BUFFERS(DP) * (2 * AtTile<DP>::BYTES + 512) + bias;   // at most 59,652 bytes
         if (a.table) {
-            MI_TRY((at_lds<&attn_dkv_kernel<DP, F16, true, 1>>(smem)));
-            MI_TRY((at_lds<&attn_dkv_kernel<DP, F16, true, 2>>(smem)));
             if (split_kv) attn_dkv_kernel<DP, F16, true, 2><<<grid, 256, smem, st>>>(a);
             else attn_dkv_kernel<DP, F16, true, 1><<<grid, 256, smem, st>>>(a);
         } else {
@@ -1550,6 +1553,8 @@ extern "C" int mi_attention_backward_dev(mi_ctx* ctx, const mi_attention_config*
     MI_TRY(fill_rows(who, "dv", dv, tokens, cfg->kv_heads, cfg->head_dim, &a.dv));
     MI_REQUIRE(tokens == 0 || lse_dev, "%s: lse is NULL (the forward pass writes it)", who);
     MI_REQUIRE(!bias_table_dev == !dbias_table_dev, "%s: dbias_table goes with bias_table", who);
+    // (the dK / dV kernel of head sizes above 64 has 512 threads a block)
+    MI_REQUIRE(cfg->head_dim <= 64 || (tokens / 128 + nseq + 10) * 8 * 512 < ((int64_t)1 << 32) - 1, "%s: %lld sequences are too many for one call", who, (long long)nseq);
     const size_t need = mi_attn_backward_bytes(a);
     MI_REQUIRE(need == 0 || (workspace_dev && ((uintptr_t)workspace_dev & 255) == 0), "%s: workspace is NULL or not 256-byte aligned", who);
     MI_REQUIRE(workspace_bytes >= need, "%s: workspace of %zu bytes, %zu are needed", who, workspace_bytes, need);
