@@ -24,7 +24,7 @@ struct mi_attn_args {
     float* parts_kv = nullptr;            // backward workspace [splits][dk | dv][tokens][key heads][hd], where splits > 1
     int splits = 1, share_heads = 1;      // shares of a group's query heads in the dK / dV kernel
     float* dtable = nullptr;              // [buckets][heads]
-    int dq_tiles = 0, dtable_x = 0;       // `partial`'s tiles; where in the dK / dV grid's x (/ 8) its blocks begin
+    int dq_tiles = 0, dtable_row = 0;     // `partial`'s tiles; the row of the dK / dV grid whose blocks sum them
     int64_t tokens = 0;
     int nseq = 0, uniform_len = 0;
     int heads = 0, group = 1, hd = 0;     // group = query heads per key head
@@ -34,7 +34,7 @@ struct mi_attn_args {
     // d < exact: d; else exact + #{t : d >= border[t]}.  From d = reach on the bucket no longer changes.
     int buckets = 0, two_sided = 0, side = 0, exact = 0, nborder = 0, reach = 0;
     int32_t border[MI_ATTN_MAX_BUCKETS + 8];   // from nborder on: beyond any distance
-    // block -> (head, tile): see attn_work in attention.hip
+    // block -> (head, tile): see at_work in attention.hip
     int tiles = 0, parts_log2 = 0, units_per_xcd = 0;
     uint32_t group_inv = 0, splits_inv = 0;   // ceil(2^32 / x), 0 for x = 1
 };

@@ -122,9 +122,10 @@ def test_backward_refused_by_its_own_arguments(kw, says):
     assert rc == -1 and says in msg, (rc, msg)
 
 
-def test_too_many_sequences_for_the_wide_backward_blocks():
-    rc, msg = _call(change=dict(head_dim=128), nseq=(1 << 20), backward=True)
-    assert rc == -1 and "too many" in msg, (rc, msg)
+def test_too_many_sequences():
+    for backward in (False, True):
+        rc, msg = _call(change=dict(head_dim=128), nseq=1 << 21, backward=backward)
+        assert rc == -1 and "too many" in msg, (rc, msg)
 
 
 def test_workspace_sizes():

@@ -29,6 +29,37 @@ def test_many_rows_under_a_key_mask(D):
     _check(x, off, lens, tab=tab, mask=mask)
 
 
+@pytest.mark.parametrize("D", [32, 128])
+def test_more_than_65535_tiles_of_a_head(D):
+    """70,000 sequences of one token (out = v, dv = dout, nothing else) around one of 70"""
+    import torch
+    from rag_amd.attention import packed_attention, packed_attention_backward
+    from tests._attention_ref import reference, worst
+    N, n = 70000, 70
+    x, _, tab = _make([N + n], 8, 8, D, table=8, seed=D)
+    off = torch.cat([torch.arange(N - 9), torch.arange(N - 9, N + 1) + n]).int().cuda()
+    assert off.shape[0] == N + 1 and int(off[-1]) == N + n
+    out, lse = packed_attention(x["q"], x["k"], x["v"], off, bias_table=tab, max_distance=20, return_lse=True)
+    dq, dk, dv, dtable = packed_attention_backward(x["dout"], x["q"], x["k"], x["v"], out, lse, off, bias_table=tab, max_distance=20)
+    torch.cuda.synchronize()
+    long = slice(N - 10, N - 9 + n)
+    part = {k: v[long] for k, v in x.items()}
+    ref = reference(part["q"], part["k"], part["v"], [n + 1], False, D ** -0.5, None, tab, 20, True, part["dout"])
+    got = {"out": out[long], "lse": lse[:, long], "dq": dq[long], "dk": dk[long], "dv": dv[long]}
+    assert all(worst(y, ref, name) <= 1.0 for name, y in got.items())
+    ones = torch.ones(N + n, dtype=torch.bool, device="cuda")
+    ones[long] = False
+    # p is rounded once on its way into the products and so is the result, 2^-8 each (backward: p is 1 to fp32's last bits); ds is
+    # the difference of two fp32 sums of D products, in either order
+    for got, want in ((out, x["v"]), (dv, x["dout"])):
+        assert bool(((got.float() - want.float()).abs()[ones] <= 2.0 ** -7 * want.float().abs()[ones]).all())
+    dp = (x["dout"].float().abs() * x["v"].float().abs()).sum(-1)
+    for got, other in ((dq, x["k"]), (dk, x["q"])):
+        assert bool((got.float().abs()[ones] <= 2.0 ** -22 * (D + 2) * dp[ones][..., None] * other.float().abs()[ones] + 1e-30).all())
+    far = torch.arange(8, device="cuda") != 0                # one-token sequences know bucket 0 alone
+    assert worst(dtable[far], {"dtable": ref["dtable"][far], "dtable_tol": ref["dtable_tol"][far]}, "dtable") <= 1.0
+
+
 def _leaves(x, tab, which):
     import torch
     t = {n: x[n].clone().requires_grad_(n in which) for n in ("q", "k", "v")}
