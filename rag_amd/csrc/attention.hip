@@ -449,8 +449,8 @@ __device__ __forceinline__ f32x16 at_first(bool near, const float* bv, int step,
 // One block per (head, 128 / KS query rows): four waves, each 32 queries by every KS-th 32-key block of the K and V tiles, which come by
 // LDS-DMA, 64 keys at a time, one barrier per tile.  With KS = 2 the two waves of a query join their sums through LDS at the end:
 // half the time per tile and twice the blocks, for calls of few blocks.  Bound: head size 128 by the products (16,384 tokens causal, 16
-// heads on 2, 1,064 us, 1,030 TFLOP/s of the 1,127 a large fp16 product reaches), 32 and 64 by the exponentials and what
-// goes with them (400 chunks up to 256 tokens, 12 heads of 32, bias: 70 us; 64 x 512 padded, 12 heads of 64: 67 us).
+// heads on 2, 1,061 us, 1,036 TFLOP/s of the 1,127 a large fp16 product reaches), 32 and 64 by the exponentials and what
+// goes with them (400 chunks up to 256 tokens, 12 heads of 32, bias: 68 us; 64 x 512 padded, 12 heads of 64: 67 us).
 template <int DP, bool F16, bool BIAS, int KS>
 __global__ __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) void attn_fwd_kernel(const mi_attn_args p)
 {
@@ -492,6 +492,10 @@ __global__ __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) void attn_fwd
     // the reference starts at a usual place and stays while the first tile's maximum lies within 2^8 of it; bf16 has fp32's range,
     // fp16 takes it 2^8 lower so that the sum is at least 1, and p up to 2^15
     constexpr float REF0 = F16 ? -8.0f : 0.0f, HIGH = F16 ? 15.0f : 8.0f, LOW = F16 ? 0.0f : -8.0f;
+    // Rows of up to 64 keys take their maximum: its p is then 1, which rounding to 16 bits leaves, and a row of one key is that key's
+    // v (sequences of a few tokens: out 1.1 - 1.2 x as far off as its own rounding alone; from the fixed reference 1.4 - 1.6; the first rows
+    // of 16,384 causal ones are half of its error, too: 1.45 -> 1.3).
+    const float high = (p.causal && qw + 32 < kend ? qw + 32 : kend) <= AT_KT ? -INFINITY : HIGH;
     float m = 0.0f, low = LOW, l = 0.0f;                               // reference = REF0 + m; low = -inf once a finite score has been seen
     bool moved = false;                                                // some lane's m is not 0
     const int R = p.reach + AT_PAD;
@@ -535,10 +539,10 @@ __global__ __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) void attn_fwd
 #pragma unroll
             for (int i = n == 0 ? 1 : 0; i + 1 < 16; i += 2) top = at_max3(top, S[n][i], S[n][i + 1]);
         top = fmaxf(top, S[0][15]);
-        if (__builtin_amdgcn_ballot_w64(top > HIGH || top < low) != 0) {
+        if (__builtin_amdgcn_ballot_w64(top > high || top < low) != 0) {
             top = fmaxf(top, at_other_half(top));                      // both halves of a query move alike
             low = fminf(low, at_other_half(low));
-            const bool move = top > HIGH || (top < low && top > -INFINITY);
+            const bool move = top > high || (top < low && top > -INFINITY);
             const float up = move ? top : 0.0f;
             const float alpha = low > -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(-up);   // (nothing summed before the first)
             m += up;
