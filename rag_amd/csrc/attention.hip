@@ -1301,8 +1301,8 @@ static int at_lds(size_t bytes)
 }
 
 // Two waves to a row where 128-row blocks are fewer than four to a CU.  Forward: 432 blocks (2 causal documents up to 4,099, 8 heads of
-// 64, bias) 76 -> 56 us, 520 (8,191, 8 heads of 128) 178 -> 160 us; 1,500 blocks (prompts up to 2,039, 32 heads of 128) 92 us
-// either way, 2,048 (16,384, 16 heads of 128) 1,066 -> 1,243 us, 8,900 (chunks up to 256, 12 heads of 32) 67 -> 83 us.  Backward: 256
+// 64, bias) 76 -> 56 us, 520 (8,191, 8 heads of 128) 178 -> 160 us; 1,500 blocks (prompts up to 2,039, 32 heads of 128) 75 ->
+// 87 us, 2,048 (16,384, 16 heads of 128) 1,066 -> 1,243 us, 8,900 (chunks up to 256, 12 heads of 32) 67 -> 83 us.  Backward: 256
 // blocks (a document of 4,000, 8 heads of 64, bias) dQ 98 -> 73 us, dK / dV 99 -> 68 us; 512 (8,191, 8 heads of 128) dQ 255 -> 228 us.
 static bool at_few(const mi_attn_args& a, int heads) { return (int64_t)heads * (a.tokens / 128 + a.nseq) < 1024; }
 
