@@ -1343,6 +1343,7 @@ int mi_launch_attention(hipStream_t st, mi_attn_args a, int dtype)
 static int at_dkv_splits(const mi_attn_args& a)
 {
     const int64_t blocks = (int64_t)(a.heads / a.group) * (a.tokens / 128 + a.nseq);
+    if (a.tokens == 0) return 1;                                       // nothing to share out, nor to join
     for (int s = 1; s < a.group; ++s)
         if (a.group % s == 0 && blocks * s >= AT_DKV_BLOCKS) return s;
     return a.group;
