@@ -42,7 +42,7 @@ def _rows(name: str, t, shape, dtype, device) -> AttentionRows:
     s = t.stride()
     if z[-1] > 1 and s[-1] != 1:
         raise ValueError(f"packed_attention: the head_dim elements of {name} must be adjacent (strides {s})")
-    if len(z) == 4 and z[0] > 1 and z[1] > 0 and s[0] != z[1] * s[1] and t.numel():
+    if len(z) == 4 and z[0] > 1 and z[1] > 1 and s[0] != z[1] * s[1] and t.numel():
         raise ValueError(f"packed_attention: the rows of {name} must be evenly spaced over the batch (strides {s})")
     # the stride of an axis of one entry is never used; what torch reports for it is arbitrary
     return AttentionRows(t.data_ptr(), s[-3] if z[-3] > 1 else (s[0] if len(z) == 4 and z[0] > 1 else z[-2] * z[-1]),

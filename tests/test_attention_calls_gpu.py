@@ -24,3 +24,19 @@ def test_empty_calls_with_grouped_heads(form, biased):
     torch.cuda.synchronize()
     assert out.shape == dq.shape == q.shape and dk.shape == dv.shape == k.shape and lse.shape == (8, 0)
     assert dtable is None if tab is None else torch.equal(dtable, torch.zeros_like(tab))
+
+
+@pytest.mark.parametrize("at", [0, 4, -1])
+def test_one_token_of_each_sequence_as_a_view(at):
+    import torch
+    from rag_amd.attention import packed_attention, packed_attention_backward
+    x, _, _ = _make([40], 4, 2, 64, seed=3)
+    y = {n: t.view(4, 10, *t.shape[1:])[:, at:at + 1 if at != -1 else None] for n, t in x.items()}
+    z = {n: t.contiguous() for n, t in y.items()}
+    assert not y["q"].is_contiguous() and y["q"].shape == (4, 1, 4, 64)
+    a = packed_attention(y["q"], y["k"], y["v"], return_lse=True)
+    b = packed_attention(z["q"], z["k"], z["v"], return_lse=True)
+    g = packed_attention_backward(y["dout"], y["q"], y["k"], y["v"], *a)
+    h = packed_attention_backward(z["dout"], z["q"], z["k"], z["v"], *b)
+    assert all(torch.equal(s, t) for s, t in zip((*a, *g[:3]), (*b, *h[:3])))
+    assert torch.equal(a[0], z["v"].repeat_interleave(2, 2))
