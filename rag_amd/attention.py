@@ -63,7 +63,7 @@ def _like(t):
 def _config(heads, kv_heads, hd, dtype, causal, scale, buckets, max_distance, bidirectional):
     if scale is None:
         scale = 1.0 / math.sqrt(hd) if hd else 1.0
-    return AttentionConfig(heads, kv_heads, hd, dtype, int(bool(causal)), 1, float(scale), buckets, int(max_distance), int(bool(bidirectional)))
+    return AttentionConfig(heads, kv_heads, hd, dtype, int(causal), 1, scale, buckets, max_distance, int(bidirectional))
 
 
 @functools.lru_cache(maxsize=256)
@@ -75,8 +75,15 @@ def _workspace(heads, kv_heads, hd, buckets, max_distance, bidirectional, tokens
     return (max(need.value, 4) + 3) // 4
 
 
+def _numbers(causal, scale, max_distance, bidirectional):
+    """As plain numbers.  Tensors and arrays of one element are numbers too, as they stand at the call: what is kept by their identity
+    (the cache of _config, an autograd node) would not see them change."""
+    return bool(causal), None if scale is None else float(scale), int(max_distance), None if bidirectional is None else bool(bidirectional)
+
+
 def _setup(q, k, v, offsets, causal, scale, key_mask, bias_table, max_distance, bidirectional):
     """(config, tokens, nseq, addresses of offsets, key_mask, bias_table) after the checks."""
+    causal, scale, max_distance, bidirectional = _numbers(causal, scale, max_distance, bidirectional)
     z, device = q.shape, q.device
     if not q.is_cuda or len(z) not in (3, 4):
         raise ValueError("packed_attention: q must be a [tokens][heads][head_dim] or [batch][length][heads][head_dim] tensor on the GPU")
@@ -131,8 +138,8 @@ def packed_attention(q, k, v, offsets=None, *, causal: bool = False, scale: Opti
 
     q [tokens][heads][head_dim], k, v [tokens][kv_heads][head_dim], bfloat16 or float16, with offsets (int32 [sequences + 1], rising
     from 0: sequence i is rows offsets[i] .. offsets[i + 1]); or [batch][length][...] without offsets.  Views are taken as they
-    are (slices of one QKV tensor).  key_mask (int32, the leading shape of q): rows that are 0 are no keys.  scale: default
-    head_dim ** -0.5.  bias_table (float32 [num_buckets][heads]) adds bias_table[bucket(key - query)]; bidirectional: buckets for
+    are (slices of one QKV tensor).  key_mask (int32, the leading shape of q): rows that are 0 are no keys.  scale: a number (not
+    differentiated), default head_dim ** -0.5.  bias_table (float32 [num_buckets][heads]) adds bias_table[bucket(key - query)]; bidirectional: buckets for
     both directions (default: not causal).  Rows that attend nothing, and rows behind the last sequence, are 0.
 
     return_lse: also the float32 [heads][tokens] log-sum-exp of each row's scores, which packed_attention_backward takes.  Runs on
@@ -140,7 +147,10 @@ def packed_attention(q, k, v, offsets=None, *, causal: bool = False, scale: Opti
 
     Differentiable once in q, k, v and bias_table under torch.autograd (out; lse is not).  A step that is captured into a graph
     calls packed_attention_backward itself: a captured backward pass of autograd may wait for streams outside the capture."""
+    if getattr(scale, "requires_grad", False) and _grad_enabled():
+        raise ValueError("packed_attention: scale is a number and has no gradient here; multiply q by what is to be learned")
     if (q.requires_grad or k.requires_grad or v.requires_grad or (bias_table is not None and bias_table.requires_grad)) and _grad_enabled():
+        causal, scale, max_distance, bidirectional = _numbers(causal, scale, max_distance, bidirectional)
         out, lse = _function().apply(q, k, v, bias_table, offsets, key_mask, causal, scale, max_distance, bidirectional)
     else:
         out, lse = _forward(q, k, v, offsets, causal, scale, key_mask, bias_table, max_distance, bidirectional, return_lse)

@@ -3,6 +3,13 @@ kernels."""
 import pytest
 
 
+def _stub(shape):
+    """What the argument checks read of a tensor on a GPU."""
+    import types
+    import torch
+    return types.SimpleNamespace(shape=torch.Size(shape), device=torch.device("cuda", 0), is_cuda=True, dtype=torch.bfloat16)
+
+
 @pytest.mark.parametrize("index", [slice(0, 1), slice(4, 5), slice(-1, None)])
 def test_a_batch_of_single_rows_may_be_a_view(index):
     """One token of each sequence of a [batch][length] tensor: rows a whole sequence apart."""
@@ -23,3 +30,36 @@ def test_views_whose_rows_are_not_evenly_spaced():
             _rows("q", v, v.shape, x.dtype, x.device)
     for v, stride in ((x[:, ::2], 2 * 256), (x[1:2, 3:7], 256), (x[1:2, :1], 256), (x[:, :, 1:3], 256)):
         assert _rows("q", v, v.shape, x.dtype, x.device).token_stride == stride
+
+
+def test_a_scale_that_is_a_tensor_counts_as_it_stands_at_the_call():
+    import numpy as np
+    import torch
+    from rag_amd.attention import _setup
+    q = _stub((2, 5, 4, 64))
+    t = torch.tensor(0.5)
+    setup = lambda scale, **kw: _setup(q, q, q, None, kw.get("causal", False), scale, None, None, kw.get("max_distance", 128), kw.get("bidirectional"))[0]   # noqa: E731
+    assert setup(t).scale == 0.5
+    t *= 2
+    assert setup(t).scale == 1.0
+    a = np.array(0.25)
+    assert setup(a).scale == 0.25
+    a[...] = 0.75
+    assert setup(a).scale == 0.75
+    causal, dist, two = torch.tensor(False), torch.tensor(100), torch.tensor(True)
+    c = setup(0.5, causal=causal, max_distance=dist, bidirectional=two)
+    assert (c.causal, c.max_distance, c.bidirectional) == (0, 100, 1)
+    causal.fill_(True), dist.fill_(200), two.fill_(False)
+    c = setup(0.5, causal=causal, max_distance=dist, bidirectional=two)
+    assert (c.causal, c.max_distance, c.bidirectional) == (1, 200, 0)
+    assert setup(None).scale == 0.125
+
+
+def test_a_scale_that_wants_a_gradient_is_refused():
+    import torch
+    from rag_amd.attention import packed_attention
+    q = torch.zeros(2, 5, 4, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="gradient"):
+        packed_attention(q, q, q, scale=torch.tensor(0.5, requires_grad=True))
+    with torch.no_grad(), pytest.raises(ValueError, match="on the GPU"):       # nothing is lost here: refused for being on the CPU
+        packed_attention(q, q, q, scale=torch.tensor(0.5, requires_grad=True))

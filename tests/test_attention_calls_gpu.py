@@ -40,3 +40,23 @@ def test_one_token_of_each_sequence_as_a_view(at):
     h = packed_attention_backward(z["dout"], z["q"], z["k"], z["v"], *b)
     assert all(torch.equal(s, t) for s, t in zip((*a, *g[:3]), (*b, *h[:3])))
     assert torch.equal(a[0], z["v"].repeat_interleave(2, 2))
+
+
+def test_a_scale_that_is_a_tensor_counts_as_it_stands_at_the_call():
+    import torch
+    from rag_amd.attention import packed_attention, packed_attention_backward
+    x, off, _ = _make([33, 80], 4, 4, 32, seed=5)
+    q, k, v = x["q"], x["k"], x["v"]
+    for device in ("cpu", "cuda"):
+        t = torch.tensor(0.25, device=device)
+        for value in (0.25, 0.5):
+            t.fill_(value)
+            assert torch.equal(packed_attention(q, k, v, off, scale=t), packed_attention(q, k, v, off, scale=value))
+    # one that changes between an autograd step's two passes: both take the first
+    out, lse = packed_attention(q, k, v, off, scale=0.5, return_lse=True)
+    want = packed_attention_backward(x["dout"], q, k, v, out, lse, off, scale=0.5)
+    leaf, t = q.clone().requires_grad_(), torch.tensor(0.5)
+    got = packed_attention(leaf, k, v, off, scale=t)
+    t.fill_(2.0)
+    got.backward(x["dout"])
+    assert torch.equal(got, out) and torch.equal(leaf.grad, want[0])
