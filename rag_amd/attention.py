@@ -17,12 +17,14 @@ from . import _capi
 from ._capi import AttentionConfig, AttentionRows
 
 
-_F32 = _I32 = _CODES = _empty_like = None
+_F32 = _I32 = _CODES = _empty_like = _grad_enabled = _forward_ad = None
 
 
 def _types():
-    global _F32, _I32, _CODES, _empty_like
+    global _F32, _I32, _CODES, _empty_like, _grad_enabled, _forward_ad
     import torch
+    import torch.autograd.forward_ad
+    _grad_enabled, _forward_ad = torch.is_grad_enabled, torch.autograd.forward_ad
     _empty_like = torch.empty_like
     _F32, _I32, _CODES = torch.float32, torch.int32, {torch.bfloat16: _capi.DTYPE_BF16, torch.float16: _capi.DTYPE_F16}
     return _CODES
@@ -79,6 +81,18 @@ def _numbers(causal, scale, max_distance, bidirectional):
     """As plain numbers.  Tensors and arrays of one element are numbers too, as they stand at the call: what is kept by their identity
     (the cache of _config, an autograd node) would not see them change."""
     return bool(causal), None if scale is None else float(scale), int(max_distance), None if bidirectional is None else bool(bidirectional)
+
+
+def _no_tangents(*tensors) -> None:
+    """Refuses tensors that carry a forward-mode tangent: they do not require a gradient, the kernels would run on their values alone
+    and the result's derivative would be zero."""
+    if _CODES is None:
+        _types()
+    if getattr(_forward_ad, "_current_level", 0) < 0:        # no such level is open
+        return
+    import torch
+    if any(isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("packed_attention: no forward-mode derivatives (torch.autograd.forward_ad); reverse mode has them")
 
 
 def _setup(q, k, v, offsets, causal, scale, key_mask, bias_table, max_distance, bidirectional):
@@ -145,8 +159,10 @@ def packed_attention(q, k, v, offsets=None, *, causal: bool = False, scale: Opti
     return_lse: also the float32 [heads][tokens] log-sum-exp of each row's scores, which packed_attention_backward takes.  Runs on
     the current stream of q's device.
 
-    Differentiable once in q, k, v and bias_table under torch.autograd (out; lse is not).  A step that is captured into a graph
+    Differentiable once in q, k, v and bias_table under torch.autograd (out; lse is not), in reverse mode: tensors with forward-mode
+    tangents are refused.  A step that is captured into a graph
     calls packed_attention_backward itself: a captured backward pass of autograd may wait for streams outside the capture."""
+    _no_tangents(q, k, v, bias_table, scale)
     if getattr(scale, "requires_grad", False) and _grad_enabled():
         raise ValueError("packed_attention: scale is a number and has no gradient here; multiply q by what is to be learned")
     if (q.requires_grad or k.requires_grad or v.requires_grad or (bias_table is not None and bias_table.requires_grad)) and _grad_enabled():
@@ -166,11 +182,6 @@ def _forward(q, k, v, offsets, causal, scale, key_mask, bias_table, max_distance
                                               _rows("k", k, zk, dtype, device), _rows("v", v, zk, dtype, device), table,
                                               _own_rows(out, z[-2], z[-1]), lse.data_ptr() if with_lse else None, _capi.stream_arg(device)))
     return out, lse
-
-
-def _grad_enabled() -> bool:
-    import torch
-    return torch.is_grad_enabled()
 
 
 def _not_captured(device) -> None:
@@ -217,6 +228,7 @@ def packed_attention_backward(dout, q, k, v, out, lse, offsets=None, *, causal: 
 
     out and lse are what packed_attention(..., return_lse=True) gave for the same arguments.  dk and dv sum over the query heads of
     a key head; rows behind the last sequence have gradient 0.  A repeated call gives the same bits."""
+    _no_tangents(dout, q, k, v, out, lse, bias_table, scale)
     cfg, tokens, nseq, off, mask, table = _setup(q, k, v, offsets, causal, scale, key_mask, bias_table, max_distance, bidirectional)
     z, zk, dtype, device = q.shape, k.shape, q.dtype, q.device
     heads = z[-2]

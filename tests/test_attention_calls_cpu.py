@@ -63,3 +63,32 @@ def test_a_scale_that_wants_a_gradient_is_refused():
         packed_attention(q, q, q, scale=torch.tensor(0.5, requires_grad=True))
     with torch.no_grad(), pytest.raises(ValueError, match="on the GPU"):       # nothing is lost here: refused for being on the CPU
         packed_attention(q, q, q, scale=torch.tensor(0.5, requires_grad=True))
+
+
+@pytest.mark.parametrize("which", ["q", "k", "v", "bias_table", "scale"])
+def test_forward_mode_derivatives_are_refused(which):
+    """A dual tensor does not require a gradient: the kernels would run on its value and drop its tangent."""
+    import torch
+    import torch.autograd.forward_ad as fwad
+    from rag_amd.attention import packed_attention
+    q = torch.zeros(2, 5, 4, 64, dtype=torch.bfloat16)
+    x = dict(q=q, k=q, v=q, bias_table=torch.zeros(32, 4), scale=torch.tensor(0.5))
+    with fwad.dual_level():
+        x[which] = fwad.make_dual(x[which], torch.ones_like(x[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            packed_attention(**x)
+        with pytest.raises(ValueError, match="on the GPU"):                    # a level alone refuses nothing
+            packed_attention(q, q, q)
+
+
+@pytest.mark.parametrize("which", ["dout", "q", "out", "lse", "bias_table"])
+def test_forward_mode_derivatives_of_the_backward_pass_are_refused(which):
+    import torch
+    import torch.autograd.forward_ad as fwad
+    from rag_amd.attention import packed_attention_backward
+    q = torch.zeros(2, 5, 4, 64, dtype=torch.bfloat16)
+    x = dict(dout=q, q=q, k=q, v=q, out=q, lse=torch.zeros(4, 10), bias_table=torch.zeros(32, 4))
+    with fwad.dual_level():
+        x[which] = fwad.make_dual(x[which].clone(), torch.ones_like(x[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            packed_attention_backward(**x)

@@ -60,3 +60,18 @@ def test_a_scale_that_is_a_tensor_counts_as_it_stands_at_the_call():
     t.fill_(2.0)
     got.backward(x["dout"])
     assert torch.equal(got, out) and torch.equal(leaf.grad, want[0])
+
+
+@pytest.mark.parametrize("which", ["q", "v", "bias_table"])
+def test_forward_mode_derivatives_are_refused(which):
+    import torch
+    import torch.autograd.forward_ad as fwad
+    from rag_amd.attention import packed_attention
+    x, off, tab = _make([33], 4, 4, 32, table=32, seed=5)
+    kw = dict(q=x["q"], k=x["k"], v=x["v"], bias_table=tab)
+    want = packed_attention(offsets=off, **kw)
+    with fwad.dual_level():
+        assert torch.equal(packed_attention(offsets=off, **kw), want)
+        kw[which] = fwad.make_dual(kw[which], torch.ones_like(kw[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            packed_attention(offsets=off, **kw)
