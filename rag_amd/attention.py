@@ -17,14 +17,19 @@ from . import _capi
 from ._capi import AttentionConfig, AttentionRows
 
 
-_F32 = _I32 = _CODES = _empty_like = _grad_enabled = _forward_ad = None
+_F32 = _I32 = _CODES = _empty_like = _grad_enabled = _forward_ad = _modes = _modes_before = _trace = None
 
 
 def _types():
-    global _F32, _I32, _CODES, _empty_like, _grad_enabled, _forward_ad
+    global _F32, _I32, _CODES, _empty_like, _grad_enabled, _forward_ad, _modes, _modes_before, _trace
     import torch
     import torch.autograd.forward_ad
     _grad_enabled, _forward_ad = torch.is_grad_enabled, torch.autograd.forward_ad
+    # whether a dispatch mode or a trace may be on at all, in tenths of a microsecond; where torch has no such name, the whole check
+    always = lambda: 1                                       # noqa: E731
+    _modes = getattr(torch._C, "_len_torch_dispatch_stack", always)
+    _modes_before = getattr(torch._ops, "_len_torch_dispatch_stack_pre_dispatch", always)
+    _trace = getattr(torch._C, "_get_tracing_state", always)
     _empty_like = torch.empty_like
     _F32, _I32, _CODES = torch.float32, torch.int32, {torch.bfloat16: _capi.DTYPE_BF16, torch.float16: _capi.DTYPE_F16}
     return _CODES
@@ -83,11 +88,17 @@ def _numbers(causal, scale, max_distance, bidirectional):
     return bool(causal), None if scale is None else float(scale), int(max_distance), None if bidirectional is None else bool(bidirectional)
 
 
-def _no_tangents(*tensors) -> None:
-    """Refuses tensors that carry a forward-mode tangent: they do not require a gradient, the kernels would run on their values alone
-    and the result's derivative would be zero."""
+def _seen_whole(*tensors) -> None:
+    """Refuses what would see a call without its kernels.  A trace (make_fx, torch.jit.trace) would hold the allocation of the result and
+    nothing that fills it.  Tensors that carry a forward-mode tangent do not require a gradient: the kernels would run on their values
+    alone and the result's derivative would be zero.  (Dispatch modes that only watch are left alone.)"""
     if _CODES is None:
         _types()
+    if _modes() or _trace() is not None or _modes_before():
+        import torch
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode
+        if torch.jit.is_tracing() or get_proxy_mode() is not None:
+            raise RuntimeError("packed_attention: under a trace (make_fx, torch.jit.trace), which would not record the kernels")
     if getattr(_forward_ad, "_current_level", 0) < 0:        # no such level is open
         return
     import torch
@@ -160,9 +171,9 @@ def packed_attention(q, k, v, offsets=None, *, causal: bool = False, scale: Opti
     the current stream of q's device.
 
     Differentiable once in q, k, v and bias_table under torch.autograd (out; lse is not), in reverse mode: tensors with forward-mode
-    tangents are refused.  A step that is captured into a graph
-    calls packed_attention_backward itself: a captured backward pass of autograd may wait for streams outside the capture."""
-    _no_tangents(q, k, v, bias_table, scale)
+    tangents are refused, and so is a call under make_fx or torch.jit.trace.  A step that is captured into a graph calls
+    packed_attention_backward itself: a captured backward pass of autograd may wait for streams outside the capture."""
+    _seen_whole(q, k, v, bias_table, scale)
     if getattr(scale, "requires_grad", False) and _grad_enabled():
         raise ValueError("packed_attention: scale is a number and has no gradient here; multiply q by what is to be learned")
     if (q.requires_grad or k.requires_grad or v.requires_grad or (bias_table is not None and bias_table.requires_grad)) and _grad_enabled():
@@ -228,7 +239,7 @@ def packed_attention_backward(dout, q, k, v, out, lse, offsets=None, *, causal: 
 
     out and lse are what packed_attention(..., return_lse=True) gave for the same arguments.  dk and dv sum over the query heads of
     a key head; rows behind the last sequence have gradient 0.  A repeated call gives the same bits."""
-    _no_tangents(dout, q, k, v, out, lse, bias_table, scale)
+    _seen_whole(dout, q, k, v, out, lse, bias_table, scale)
     cfg, tokens, nseq, off, mask, table = _setup(q, k, v, offsets, causal, scale, key_mask, bias_table, max_distance, bidirectional)
     z, zk, dtype, device = q.shape, k.shape, q.dtype, q.device
     heads = z[-2]

@@ -92,3 +92,24 @@ def test_forward_mode_derivatives_of_the_backward_pass_are_refused(which):
         x[which] = fwad.make_dual(x[which].clone(), torch.ones_like(x[which]))
         with pytest.raises(RuntimeError, match="forward-mode"):
             packed_attention_backward(**x)
+
+
+@pytest.mark.parametrize("backward", [False, True])
+@pytest.mark.parametrize("how", ["make_fx", "make_fx pre_dispatch", "jit.trace"])
+def test_tracing_is_refused(how, backward):
+    """A trace would hold the allocation of the result and not the kernel that fills it."""
+    import torch
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from rag_amd.attention import packed_attention, packed_attention_backward
+    q, lse = torch.zeros(2, 5, 4, 64, dtype=torch.bfloat16), torch.zeros(4, 10)
+
+    def f(x):
+        return packed_attention_backward(x, x, x, x, x, lse)[0] if backward else packed_attention(x, x, x)
+
+    with pytest.raises(RuntimeError, match="trac"):
+        if how == "jit.trace":
+            torch.jit.trace(f, q, check_trace=False)
+        else:
+            make_fx(f, pre_dispatch=how.endswith("dispatch"))(q)
+    with pytest.raises(ValueError, match="on the GPU"):                        # and afterwards as before
+        f(q)

@@ -75,3 +75,16 @@ def test_forward_mode_derivatives_are_refused(which):
         kw[which] = fwad.make_dual(kw[which], torch.ones_like(kw[which]))
         with pytest.raises(RuntimeError, match="forward-mode"):
             packed_attention(offsets=off, **kw)
+
+
+def test_tracing_is_refused():
+    import torch
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from rag_amd.attention import packed_attention
+    x, off, _ = _make([33], 4, 4, 32, seed=5)
+    f = lambda q: packed_attention(q, x["k"], x["v"], off)                       # noqa: E731
+    with pytest.raises(RuntimeError, match="trac"):
+        make_fx(f)(x["q"])
+    with pytest.raises(RuntimeError, match="trac"):
+        torch.jit.trace(f, x["q"], check_trace=False)
+    assert torch.equal(f(x["q"]), f(x["q"]))
