@@ -306,12 +306,15 @@ int  mi_encoder_last_time(const mi_encoder* enc, float* out_ms);
  * sentence-transformers, advanced_rag.py:104-107); the encoder calls it for models that are causal or carry such a bias
  * (mi_encoder_set_attention).
  *
- *   s_ij = scale * q_i . k_j + bias_table[bucket(j - i)][head],  p = softmax over the attended j,  out_i = sum_j p_ij v_j
+ *   s_ij = scale * q_i . k_j + b_ij,  b_ij = bias_table[bucket(j - i)][head], where finite at most 4096 in size,
+ *   p = softmax of s over the attended j,  out_i = sum_j p_ij v_j
  *
  * over rows i, j of one sequence; j is attended when it is a key (key_mask, if given, is not 0 there) and, with `causal`,
  * j <= i.  Query head h reads key head h / (heads / kv_heads).  A row that attends nothing has out = 0 and lse = -inf.
  *
- * A finite bias counts as at most 4096 in size; -inf takes its bucket's keys out.
+ * A finite bias counts as at most 4096 in size, with its sign: beyond that it only says "never" or "always" beside keys of another
+ * bias, and keys whose biases are beyond it on the same side count alike (-5000 as much as -6000).  dbias_table is the gradient in the
+ * bias as it counts (not cut to 0 beyond the bound).  -inf takes its bucket's keys out.
  *
  * bucket(r), the scheme of relative-position encoders: bidirectional: n = num_buckets / 2, d = |r|, and n is added for r > 0;
  * otherwise n = num_buckets, d = max(-r, 0).  With m = n / 2 the distances d < m have a bucket each, then

@@ -1,6 +1,7 @@
 """Packed attention as an operator on torch tensors (mi_attention_dev, mi_attention_backward_dev): whole sequences of different
 lengths back to back, or a padded batch under a key mask; causal or not; grouped key / value heads; a relative position bias
-learned by buckets.  The formulas and the limits stand in include/mi355rag.h.  Everything numeric runs in
+learned by buckets (a finite bias counts as at most 4096 in size, here and in the gradients).  The formulas and the limits stand in
+include/mi355rag.h.  Everything numeric runs in
 rag_amd/lib/libmi355rag.so on an MI355X; there is no CPU fallback.
 
     out = packed_attention(q, k, v, offsets, causal=True)              # q [tokens][heads][head_dim], k / v [tokens][kv_heads][head_dim]
@@ -159,13 +160,15 @@ def relative_position_buckets(rel, num_buckets: int, max_distance: int = 128, bi
 
 def packed_attention(q, k, v, offsets=None, *, causal: bool = False, scale: Optional[float] = None, key_mask=None,
                      bias_table=None, max_distance: int = 128, bidirectional: Optional[bool] = None, return_lse: bool = False):
-    """softmax(scale * q k^T + bias) v over the rows of each sequence.
+    """softmax(scale * q k^T + bias) v over the rows of each sequence, bias being the table's value or, where a finite one is larger in
+    size, 4096 with its sign.
 
     q [tokens][heads][head_dim], k, v [tokens][kv_heads][head_dim], bfloat16 or float16, with offsets (int32 [sequences + 1], rising
     from 0: sequence i is rows offsets[i] .. offsets[i + 1]); or [batch][length][...] without offsets.  Views are taken as they
     are (slices of one QKV tensor).  key_mask (int32, the leading shape of q): rows that are 0 are no keys.  scale: a number (not
-    differentiated), default head_dim ** -0.5.  bias_table (float32 [num_buckets][heads]) adds bias_table[bucket(key - query)]; bidirectional: buckets for
-    both directions (default: not causal).  Rows that attend nothing, and rows behind the last sequence, are 0.
+    differentiated), default head_dim ** -0.5.  bias_table (float32 [num_buckets][heads]) adds
+    bias_table[bucket(key - query)]; bidirectional: buckets for both directions (default: not causal).  Rows that attend nothing, and
+    rows behind the last sequence, are 0.
 
     return_lse: also the float32 [heads][tokens] log-sum-exp of each row's scores, which packed_attention_backward takes.  Runs on
     the current stream of q's device.
@@ -238,7 +241,8 @@ def packed_attention_backward(dout, q, k, v, out, lse, offsets=None, *, causal: 
     """Gradients of sum(dout * packed_attention(q, k, v, ...)): (dq, dk, dv, dbias_table), the last None without a bias_table.
 
     out and lse are what packed_attention(..., return_lse=True) gave for the same arguments.  dk and dv sum over the query heads of
-    a key head; rows behind the last sequence have gradient 0.  A repeated call gives the same bits."""
+    a key head; rows behind the last sequence have gradient 0.  dbias_table is the gradient in the bias as it counts: the bound of
+    4096 passes it through.  A repeated call gives the same bits."""
     _seen_whole(dout, q, k, v, out, lse, bias_table, scale)
     cfg, tokens, nseq, off, mask, table = _setup(q, k, v, offsets, causal, scale, key_mask, bias_table, max_distance, bidirectional)
     z, zk, dtype, device = q.shape, k.shape, q.dtype, q.device

@@ -101,7 +101,8 @@ class Encoder:
 
     def set_attention(self, causal: bool = False, bias_table=None, max_distance: int = 128, bidirectional: Optional[bool] = None) -> None:
         """Attention of the layers: causal, and / or with a relative position bias learned by buckets (bias_table [num_buckets][heads],
-        shared by the layers; bidirectional: buckets for both directions, default: not causal), as packed_attention computes it.
+        shared by the layers; bidirectional: buckets for both directions, default: not causal), as packed_attention computes it (a finite
+        bias counts as at most 4096 in size).
         Without arguments: the built-in attention again."""
         table, buckets = None, 0
         if bias_table is not None:

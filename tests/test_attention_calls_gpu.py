@@ -88,3 +88,22 @@ def test_tracing_is_refused():
     with pytest.raises(RuntimeError, match="trac"):
         torch.jit.trace(f, x["q"], check_trace=False)
     assert torch.equal(f(x["q"]), f(x["q"]))
+
+
+def test_a_finite_bias_counts_as_at_most_4096():
+    """The stated bound: -5,000 and -6,000 are both -4,096, whichever other keys a row has, and the gradient is the table's as it counts."""
+    import torch
+    from rag_amd.attention import packed_attention, packed_attention_backward
+    lens = [40, 7]
+    for D in (32, 64, 128):
+        x, off, tab = _make(lens, 4, 2, D, table=8, seed=D)
+        tab[0, :2], tab[1:4, :2], tab[5:, :2] = -5000.0, -6000.0, -1e30
+        tab[0, 2], tab[2, 2] = 5000.0, 1e30
+        kept = tab.clamp(-4096, 4096)
+        assert not torch.equal(kept, tab)
+        res = []
+        for t in (tab, kept):
+            out, lse = packed_attention(x["q"], x["k"], x["v"], off, bias_table=t, max_distance=20, return_lse=True)
+            res.append((out, lse, *packed_attention_backward(x["dout"], x["q"], x["k"], x["v"], out, lse, off, bias_table=t, max_distance=20)))
+        assert all(torch.equal(a, b) for a, b in zip(*res))
+        _check(x, off, lens, tab=tab, max_distance=20)
