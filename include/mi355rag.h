@@ -328,7 +328,8 @@ int  mi_encoder_last_time(const mi_encoder* enc, float* out_ms);
  * zero_tail, set to 0 (lse: -inf).  Values of one sequence never reach another, and rows that key_mask takes out may hold
  * anything in k and v; a NaN or infinity in a row reaches the rows of its own sequence that attend it, and with `causal` may also
  * reach earlier rows of that sequence.
- * Softmax statistics and sums are fp32; p (and, backward, ds) is rounded to the tensors' type for the matrix product. */
+ * Softmax statistics and sums are fp32; p (and, backward, ds) is rounded to the tensors' type for the matrix product, in fp16 times a
+ * power of two that keeps small and large ones in the type's normal range. */
 typedef struct {
     int32_t heads, kv_heads;          /* heads a multiple of kv_heads */
     int32_t head_dim;

@@ -647,6 +647,56 @@ __global__ __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) void attn_fwd
 // thousands of keys has p near fp16's subnormals), and ds = p (dp - D) takes the scale back out.
 template <bool F16> struct AtPScale { static constexpr float log2 = F16 ? 12.0f : 0.0f, down = F16 ? 1.0f / 4096.0f : 1.0f; };
 
+// the largest of a block's 16 sizes (three steps deep: as one chain of eight it held up the short calls)
+__device__ __forceinline__ float at_size(const f32x16& x)
+{
+    float m[5];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) m[i] = at_max3(fabsf(x[3 * i]), fabsf(x[3 * i + 1]), fabsf(x[3 * i + 2]));
+    return fmaxf(at_max3(m[0], m[1], m[2]), at_max3(m[3], m[4], fabsf(x[15])));
+}
+
+// The power of two that ds is carried with into the 16-bit operand of dQ and dK, fp16 only: with dout as a loss's mean leaves it (1e-3,
+// 4,096 keys) ds lies in fp16's subnormals and its rounding was 8 times the result's own; with large v and dout it is beyond 65,504.  One
+// power for each lane's sum (a query's dQ, a key's dK).  It starts where no ds that counts is lost, and where a block's largest would pass
+// 2^15 with it, it falls to put that at 2^10 .. 2^11: at a lane's first block, and then for a ds 2^5 times as large as any before.  So a ds
+// is off by 2^-11 of itself or by 2^-35 of the lane's largest.  (Bounded by |dp - D| instead, which is there earlier, the rows and keys
+// whose p are all tiny would lose theirs.)  bf16 has fp32's range and does without.  The check costs the fp16 kernels 1 - 7 % (24 passages up
+// to 511, 12 heads of 64, bias: dQ 62.5 -> 64.6 us, dK / dV 40.5 -> 41.8; 9 prompts up to 2,048, 16 heads on 4 of 128: 117 -> 121).
+template <bool F16> struct AtDsScale {
+    static constexpr float START = F16 ? 0x1p60f : 1.0f;               // (|dp| < 2^41: finite)
+    float up = START;
+    // ds: N blocks, times `up` already.  What the lane has summed goes along, and also(f) takes the change to what makes the next ds.
+    template <int N, int M, class Also>
+    __device__ __forceinline__ void fit(f32x16 (&ds)[N], f32x16 (&sum)[M], Also&& also)
+    {
+        if constexpr (F16) {
+            float top = at_size(ds[0]);
+#pragma unroll
+            for (int n = 1; n < N; ++n) top = fmaxf(top, at_size(ds[n]));
+            if (__builtin_amdgcn_ballot_w64(top > 0x1p15f) != 0) {
+                top = fmaxf(top, at_other_half(top));                  // both halves of a lane's sum move alike
+                const float f = top > 0x1p15f && top < INFINITY ? __builtin_amdgcn_ldexpf(0x1p11f, -__builtin_amdgcn_frexp_expf(top)) : 1.0f;
+                up *= f;
+#pragma unroll
+                for (int n = 0; n < N; ++n) ds[n] = ds[n] * f;
+#pragma unroll
+                for (int m = 0; m < M; ++m) sum[m] = sum[m] * f;
+                also(f);
+            }
+        }
+    }
+    // the sum without the power
+    template <int M> __device__ __forceinline__ void down(f32x16 (&sum)[M], float f = 1.0f) const
+    {
+        if constexpr (F16) {
+            f /= up;
+#pragma unroll
+            for (int m = 0; m < M; ++m) sum[m] = sum[m] * f;
+        }
+    }
+};
+
 #define AT_DQ_BUFFERS(DP, BIAS) ((BIAS) ? ((DP) == 32 ? 3 : 2) : AT_BUFFERS(DP))
 // dQ: one block per (head, 128 query rows), like the forward pass: S^T = K Q^T and dP^T = V dO^T with the query on the lane,
 // dQ^T += K^T dS^T, with ds = p (dp - D).
@@ -793,13 +843,19 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const mi_attn_args p)
         p.lse2[(int64_t)head * p.tokens + tok] = nl;
     }
 
-    const float Df = D * fix;
+    // ds = p fix (dp - D), times the power of two but with a bias.  LATE: `fix` waits for the end, in LDS: a register more would leave head
+    // size 64 two blocks a CU (100 x 512, 12 heads: 175 -> 219 us).
+    AtDsScale<F16> sc;
+    constexpr bool LATE = F16 && !BIAS && KS == 1;
+    if constexpr (LATE) pair[wave][0][lane] = fix;
+    else if constexpr (F16 && !BIAS) fix *= sc.START;
+    float Df = LATE ? D * sc.START : D * fix;
     f32x16 dQ[DP / 32];
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) dQ[dt] = at_zero16();
     walk([&](const char* Kt, int st, const f32x16& S, f32x16& dP, bool near, int rlo, int rhi) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) dP[i] = S[i] * __builtin_fmaf(dP[i], fix, -Df);   // ds
+        for (int i = 0; i < 16; ++i) dP[i] = S[i] * __builtin_fmaf(dP[i], LATE ? sc.up : fix, -Df);   // ds
         if constexpr (BIAS) {
             if (near) {
                 float* const at = skew + col * 63 + 31 + 4 * half;
@@ -817,15 +873,23 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const mi_attn_args p)
                 farS[1] += rhi <= -p.reach ? 0.0f : sum[0] + sum[1];
             }
         }
+        f32x16 ds[1] = {F16 && BIAS ? dP * sc.up : dP};                // (the table's sums take it as it is)
+        sc.fit(ds, dQ, [&](float f) __attribute__((always_inline)) {
+            if constexpr (!BIAS) {
+                if constexpr (!LATE) fix *= f;
+                Df *= f;
+            }
+        });
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
             u32x4 sf;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sf[i] = at_pack2<F16>(dP[8 * kk + 2 * i], dP[8 * kk + 2 * i + 1]);
+            for (int i = 0; i < 4; ++i) sf[i] = at_pack2<F16>(ds[0][8 * kk + 2 * i], ds[0][8 * kk + 2 * i + 1]);
 #pragma unroll
             for (int dt = 0; dt < DP / 32; ++dt) dQ[dt] = at_mfma<F16>(at_cols<DP>(Kt, 2 * st + kk, dt, lane), sf, dQ[dt]);
         }
     });
+    sc.down(dQ, LATE ? pair[wave][0][lane] : 1.0f);
     if constexpr (KS == 2) {
         at_sync();
         float* const x = reinterpret_cast<float*>(lds) + (wave & 1) * (DP / 2) * 64 + lane;
@@ -961,6 +1025,9 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const mi_attn_args p)
     f32x16 dK[DP / 32], dV[DP / 32];
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) { dK[dt] = at_zero16(); dV[dt] = at_zero16(); }
+    AtDsScale<F16> sc;
+    float dsf = AtPScale<F16>::down * sc.START;                        // ds = (p 2^12) (dp - D) dsf
+    if (F16 && !on) dsf = 0.0f;                                        // a masked key: whatever its p, nothing to keep in range
 #pragma unroll
     for (int t2 = 0; t2 < NB - 1; ++t2) if (t2 < n) issue(t2);
     const int R = p.reach + AT_PAD;
@@ -992,7 +1059,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const mi_attn_args p)
 #pragma unroll
         for (int st = s0; st < (KS == 1 ? 2 : s0 + 1); ++st) {
             if ((q0 + 32 * st >= len || (p.causal && q0 + 32 * st + 31 < kw))) continue;
-            f32x16 S = at_first<F16>(near, vec + at - 32 * st, -1, at_rows<DP>(Qt, st, 0, col, half), kf[0]), dP = at_zero16();
+            f32x16 S = at_first<F16>(near, vec + at - 32 * st, -1, at_rows<DP>(Qt, st, 0, col, half), kf[0]), X[1] = {at_zero16()};
+            f32x16& dP = X[0];
 #pragma unroll
             for (int s = 1; s < DP / 16; ++s) S = at_mfma<F16>(at_rows<DP>(Qt, st, s, col, half), kf[s], S);
 #pragma unroll
@@ -1006,7 +1074,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const mi_attn_args p)
                 for (int e = 0; e < 4; ++e) {
                     const int i = 4 * g + e;
                     S[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], p.scale_log2, add - nls[e]));
-                    dP[i] = S[i] * ((dP[i] - Drs[e]) * AtPScale<F16>::down);
+                    dP[i] = S[i] * ((dP[i] - Drs[e]) * dsf);
                 }
             }
             if ((p.causal && q0 + 32 * st < kw + 31) || q0 + 32 * st + 32 > len) {   // rows that do not attend, or are none
@@ -1019,6 +1087,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const mi_attn_args p)
                     dP[i] = ok ? dP[i] : 0.0f;
                 }
             }
+            sc.fit(X, dK, [&](float f) __attribute__((always_inline)) { dsf *= f; });
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
                 u32x4 pf, sf;
@@ -1035,6 +1104,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const mi_attn_args p)
             }
         }
     }
+    sc.down(dK);
     if constexpr (KS == 2) {
         at_sync();
         float* const x = reinterpret_cast<float*>(lds) + (wave & 1) * DP * 64 + lane;
@@ -1160,15 +1230,19 @@ __global__ __launch_bounds__(512, 2) void attn_dkv_pair_kernel(const mi_attn_arg
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    auto sum_up = [&](const char* rows_t, const f32x16 (&X)[2]) __attribute__((always_inline)) {
+    auto sum_half = [&](const char* rows_t, int st, const f32x16& X) __attribute__((always_inline)) {
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
+        for (int kk = 0; kk < 2; ++kk) {
             u32x4 f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = at_pack2<F16>(X[kk >> 1][8 * (kk & 1) + 2 * i], X[kk >> 1][8 * (kk & 1) + 2 * i + 1]);
+            for (int i = 0; i < 4; ++i) f[i] = at_pack2<F16>(X[8 * kk + 2 * i], X[8 * kk + 2 * i + 1]);
 #pragma unroll
-            for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = at_mfma<F16>(at_cols<DP>(rows_t, kk, dt, lane), f, acc[dt]);
+            for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = at_mfma<F16>(at_cols<DP>(rows_t, 2 * st + kk, dt, lane), f, acc[dt]);
         }
+    };
+    auto sum_up = [&](const char* rows_t, const f32x16 (&X)[2]) __attribute__((always_inline)) {
+        sum_half(rows_t, 0, X[0]);
+        sum_half(rows_t, 1, X[1]);
     };
     float4* const mine = pass + pair * 8 * 64 + lane;
     if (first) {
@@ -1208,6 +1282,9 @@ __global__ __launch_bounds__(512, 2) void attn_dkv_pair_kernel(const mi_attn_arg
             if (!idle) sum_up(Qt + TB, S);
         }
     } else {
+        AtDsScale<F16> sc;
+        float dsf = AtPScale<F16>::down * sc.START;                    // as in attn_dkv_kernel
+        if (F16 && !on) dsf = 0.0f;
         for (int it = 0; it < n; ++it) {
             const char* const Qt = next(it);
             const bool idle = kw >= len || (p.causal && q0 + AT_KT - 1 < kw);
@@ -1217,9 +1294,40 @@ __global__ __launch_bounds__(512, 2) void attn_dkv_pair_kernel(const mi_attn_arg
                 for (int st = 0; st < 2; ++st)
 #pragma unroll
                     for (int s = 0; s < DP / 16; ++s) dP[st] = at_mfma<F16>(at_rows<DP>(Qt + TB, st, s, col, half), wf[s], s == 0 ? at_zero16() : dP[st]);
+                if constexpr (F16) {
+#pragma unroll
+                    for (int st = 0; st < 2; ++st)
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            const float4 Dr = *reinterpret_cast<const float4*>(rowv + buf * 128 + 64 + 32 * st + 8 * g + 4 * half);
+                            const float Drs[4] = {Dr.x, Dr.y, Dr.z, Dr.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) dP[st][4 * g + e] = (dP[st][4 * g + e] - Drs[e]) * dsf;
+                        }
+                }
             }
             there();
-            if (!idle) {
+            if constexpr (F16) {
+                // the power of two is looked after 32 rows at a time, so that one half's products run beside the other's check
+                if (!idle) {
+#pragma unroll
+                    for (int st = 0; st < 2; ++st) {
+                        f32x16 x[1];
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            const float4 P = mine[(4 * st + g) * 64];
+                            const float Ps[4] = {P.x, P.y, P.z, P.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) x[0][4 * g + e] = Ps[e] * dP[st][4 * g + e];
+                        }
+                        sc.fit(x, acc, [&](float f) __attribute__((always_inline)) {
+                            dsf *= f;
+                            if (st == 0) dP[1] = dP[1] * f;
+                        });
+                        sum_half(Qt, st, x[0]);
+                    }
+                }
+            } else if (!idle) {
 #pragma unroll
                 for (int st = 0; st < 2; ++st)
 #pragma unroll
@@ -1232,6 +1340,7 @@ __global__ __launch_bounds__(512, 2) void attn_dkv_pair_kernel(const mi_attn_arg
                 sum_up(Qt, dP);
             }
         }
+        sc.down(acc);
     }
     if (key < len) {
         if (!on) {                                                     // a masked key (the products above ran on its column alone)
