@@ -10,6 +10,15 @@ from tests.test_attention_gpu import _check, _make
 pytestmark = pytest.mark.gpu
 
 
+def _splits(H, Hk, D, tokens, nseq):
+    """Into how many shares the backward pass divides a group's query heads, read off the workspace it asks for."""
+    from rag_amd import _capi
+    need = ctypes.c_size_t()
+    cfg = _capi.AttentionConfig(H, Hk, D, _capi.DTYPE_BF16, 0, 1, 1.0, 0, 0, 0)
+    _capi.check(_capi.load().mi_attention_backward_workspace(cfg, tokens, nseq, 1, ctypes.byref(need)))
+    return max(1, (need.value - H * tokens * 8) // (2 * tokens * Hk * D * 4))
+
+
 @pytest.mark.parametrize("biased", [False, True])
 @pytest.mark.parametrize("form", ["no sequence", "empty sequences", "empty batch", "sequences of no rows"])
 def test_empty_calls_with_grouped_heads(form, biased):
@@ -40,6 +49,36 @@ def test_one_token_of_each_sequence_as_a_view(at):
     h = packed_attention_backward(z["dout"], z["q"], z["k"], z["v"], *b)
     assert all(torch.equal(s, t) for s, t in zip((*a, *g[:3]), (*b, *h[:3])))
     assert torch.equal(a[0], z["v"].repeat_interleave(2, 2))
+
+
+@pytest.mark.parametrize("H,Hk,repeats,splits", [(8, 4, 44, 1), (16, 4, 25, 2), (32, 16, 12, 1)])
+@pytest.mark.parametrize("table", [0, 32])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("D,dtype", [(32, "bf16"), (64, "fp16"), (128, "bf16"), (128, "fp16")])
+def test_blocks_that_walk_several_query_heads(D, dtype, causal, table, H, Hk, repeats, splits):
+    """Large batches of grouped heads: a dK / dV block takes group / splits > 1 query heads one after another.  The batch repeats a
+    pattern of sequences, so that the 64-bit form is worked out for one: a repeat's results are the first's, bit for bit, and the
+    table's gradient is the sum of the repeats'."""
+    import torch
+    from rag_amd.attention import packed_attention, packed_attention_backward
+    lens = [200, 1, 0, 64, 130, 33, 7, 129]
+    T = sum(lens)
+    assert _splits(H, Hk, D, T * repeats, len(lens) * repeats) == splits < H // Hk
+    x, _, tab = _make(lens, H, Hk, D, dtype, table=table, seed=D + H + causal)
+    many = {n: t.repeat(repeats, 1, 1) for n, t in x.items()}
+    off = torch.tensor([0] + lens * repeats, dtype=torch.int32).cumsum(0).to(torch.int32).cuda()
+    kw = dict(causal=causal, bias_table=tab, max_distance=64)
+    out, lse = packed_attention(many["q"], many["k"], many["v"], off, return_lse=True, **kw)
+    dq, dk, dv, dtable = packed_attention_backward(many["dout"], many["q"], many["k"], many["v"], out, lse, off, **kw)
+    torch.cuda.synchronize()
+    ref = reference(x["q"], x["k"], x["v"], lens, causal, D ** -0.5, None, tab, 64, not causal, x["dout"])
+    for n, t in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv)):
+        t = t.view(repeats, T, *t.shape[1:])
+        assert torch.equal(t, t[:1].expand_as(t)), n
+        assert worst(t[0], ref, n) <= 1.0, n
+    assert worst(lse[:, :T], ref, "lse") <= 1.0
+    if table:
+        assert worst(dtable / repeats, ref, "dtable") <= 1.0
 
 
 def test_a_scale_that_is_a_tensor_counts_as_it_stands_at_the_call():
