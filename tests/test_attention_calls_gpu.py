@@ -81,6 +81,58 @@ def test_blocks_that_walk_several_query_heads(D, dtype, causal, table, H, Hk, re
         assert worst(dtable / repeats, ref, "dtable") <= 1.0
 
 
+def _long_mask(L, seed):
+    """Whole tiles of 64 keys in front (past the 64th), a stretch without keys, holes on both sides of tile 256, none in the last tiles."""
+    import torch
+    m = (torch.rand(L, generator=torch.Generator().manual_seed(seed)) < 0.6).int()
+    m[:64 * 66 + 5] = 1
+    m[64 * 66 + 5:64 * 68] = 0
+    if L > 64 * 257:
+        m[64 * 255 - 3:64 * 257 + 9] = 0
+        m[64 * 255 + 20] = m[64 * 256 + 3] = 1
+    m[L - 100:] = 0
+    return m.cuda()
+
+
+@pytest.mark.parametrize("causal,table", [(False, 0), (True, 32)])
+@pytest.mark.parametrize("L", [4096 + 300, 16384 + 333])
+def test_a_key_mask_over_many_tiles(L, causal, table):
+    """Past 64 tiles a block scans its words in rounds, past 256 it reads the mask as it goes."""
+    import torch
+    x, off, tab = _make([L], 2, 1, 32, table=table, seed=L)
+    mask = _long_mask(L, 7)
+    assert int(mask.sum()) > L // 2
+    for n in ("k", "v"):
+        x[n][mask == 0] = float("nan")
+    got, _ = _check(x, off, [L], tab=tab, mask=mask, causal=causal)
+    assert torch.all(got["dk"][mask == 0] == 0) and torch.all(got["dv"][mask == 0] == 0)
+
+
+@pytest.mark.parametrize("H,Hk", [(4, 4), (8, 2)])
+@pytest.mark.parametrize("D,dtype", [(32, "fp16"), (64, "bf16"), (128, "bf16")])
+@pytest.mark.parametrize("biased", [False, True])
+def test_padded_batch_causal_and_grouped(biased, D, dtype, H, Hk):
+    import torch
+    from rag_amd.attention import packed_attention, packed_attention_backward
+    B, L = 5, 150
+    x, _, tab = _make([L] * B, H, Hk, D, dtype, table=32 if biased else 0, seed=D)
+    at = torch.arange(L)[None, :]
+    km = ((at < torch.tensor([150, 3, 70, 0, 64])[:, None]) & (at >= torch.tensor([0, 0, 5, 0, 1])[:, None])).int().cuda()   # also padded in front
+    for n in ("k", "v"):
+        x[n][km.view(-1) == 0] = float("nan")
+    y = {n: t.view(B, L, *t.shape[1:]) for n, t in x.items()}
+    kw = dict(causal=True, key_mask=km, bias_table=tab)
+    out, lse = packed_attention(y["q"], y["k"], y["v"], return_lse=True, **kw)
+    grads = packed_attention_backward(y["dout"], y["q"], y["k"], y["v"], out, lse, **kw)
+    ref = reference(x["q"], x["k"], x["v"], [L] * B, True, D ** -0.5, km.view(-1), tab, 128, False, x["dout"])
+    got = {"out": out.view(-1, H, D), "lse": lse, **{n: t.view(-1, t.shape[-2], D) for n, t in zip(("dq", "dk", "dv"), grads)}}
+    if biased:
+        got["dtable"] = grads[3]
+    off_by = {n: worst(t, ref, n) for n, t in got.items()}
+    assert all(v <= 1.0 for v in off_by.values()), off_by
+    assert torch.all(out[2, :5] == 0) and torch.all(grads[0][2, :5] == 0)
+
+
 def test_a_scale_that_is_a_tensor_counts_as_it_stands_at_the_call():
     import torch
     from rag_amd.attention import packed_attention, packed_attention_backward
