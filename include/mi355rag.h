@@ -356,8 +356,8 @@ int  mi_attention_buckets(int num_buckets, int max_distance, int bidirectional, 
 /* Gradients of sum(dout * out): dq, dk, dv (rows as above; dk and dv are the sums over a group's query heads), and, with a
  * bias, dbias_table fp32 [num_buckets][heads] (overwritten, not added to).  out and lse are the forward pass's.  The results of
  * a repeated call are the same bits: nothing is summed by atomics in an order of its own.  workspace_dev: 256-byte aligned,
- * mi_attention_backward_workspace bytes (packed: offsets are given), the caller's alone until the work on the stream is done.
- * dq, dk, dv overlap no input. */
+ * mi_attention_backward_workspace bytes (packed: offsets are given; it refuses the sizes that the call does), the caller's alone
+ * until the work on the stream is done.  dq, dk, dv overlap no input. */
 int  mi_attention_backward_workspace(const mi_attention_config* cfg, int64_t tokens, int64_t nseq, int packed, size_t* bytes);
 int  mi_attention_backward_dev(mi_ctx* ctx, const mi_attention_config* cfg, int64_t tokens, int64_t nseq,
                                const int32_t* offsets_dev, const int32_t* key_mask_dev, const mi_attention_rows* q,

@@ -1576,6 +1576,27 @@ static int fill_rows(const char* who, const char* what, const mi_attention_rows*
     return MI_OK;
 }
 
+// What a call's sizes have to be, for its workspace as for the call.
+static int check_heads(const char* who, const mi_attention_config* c)
+{
+    MI_REQUIRE(c->heads > 0 && c->heads <= 65535 && c->kv_heads > 0 && c->heads % c->kv_heads == 0, "%s: heads %d must be a positive multiple of kv_heads %d", who, c->heads, c->kv_heads);
+    MI_REQUIRE(c->head_dim > 0 && c->head_dim % 8 == 0 && c->head_dim <= 128, "%s: head_dim %d must be a multiple of 8 up to 128", who, c->head_dim);
+    return MI_OK;
+}
+static int check_rows(const char* who, int64_t tokens, int64_t nseq, bool packed)
+{
+    MI_REQUIRE(tokens >= 0 && tokens < ((int64_t)1 << 31) - 4096, "%s: %lld tokens out of range", who, (long long)tokens);
+    MI_REQUIRE(nseq >= 0 && nseq < ((int64_t)1 << 24), "%s: %lld sequences out of range", who, (long long)nseq);
+    MI_REQUIRE(packed || (nseq == 0 ? tokens == 0 : tokens % nseq == 0), "%s: %lld tokens are not %lld sequences of one length", who, (long long)tokens, (long long)nseq);
+    return MI_OK;
+}
+static int check_launch(const char* who, const mi_attention_config* c, int64_t tokens, int64_t nseq)
+{
+    // one launch: fewer than 2^21 tiles of a head (of at least 64 rows each), 2^31 blocks
+    MI_REQUIRE(tokens / 64 + nseq + 9 < ((int64_t)1 << 21) && (tokens / 64 + nseq + 9) * (int64_t)c->heads < ((int64_t)1 << 31) - 1, "%s: %lld tokens in %lld sequences x %d heads are too many for one call", who, (long long)tokens, (long long)nseq, c->heads);
+    return MI_OK;
+}
+
 // Everything both directions check; fills the fields they share.
 static int fill_args(const char* who, mi_ctx* ctx, const mi_attention_config* c, int64_t tokens, int64_t nseq, const int32_t* offsets,
                      const int32_t* key_mask, const mi_attention_rows* q, const mi_attention_rows* k, const mi_attention_rows* v,
@@ -1583,12 +1604,9 @@ static int fill_args(const char* who, mi_ctx* ctx, const mi_attention_config* c,
 {
     MI_REQUIRE(ctx && c, "%s: NULL argument", who);
     MI_REQUIRE(c->dtype == MI_DTYPE_BF16 || c->dtype == MI_DTYPE_F16, "%s: dtype %d is not MI_DTYPE_BF16 or MI_DTYPE_F16", who, c->dtype);
-    MI_REQUIRE(c->heads > 0 && c->heads <= 65535 && c->kv_heads > 0 && c->heads % c->kv_heads == 0, "%s: heads %d must be a positive multiple of kv_heads %d", who, c->heads, c->kv_heads);
-    MI_REQUIRE(c->head_dim > 0 && c->head_dim % 8 == 0 && c->head_dim <= 128, "%s: head_dim %d must be a multiple of 8 up to 128", who, c->head_dim);
+    MI_TRY(check_heads(who, c));
     MI_REQUIRE(c->scale >= 1e-20f && c->scale <= 1e20f, "%s: scale must be between 1e-20 and 1e20", who);
-    MI_REQUIRE(tokens >= 0 && tokens < ((int64_t)1 << 31) - 4096, "%s: %lld tokens out of range", who, (long long)tokens);
-    MI_REQUIRE(nseq >= 0 && nseq < ((int64_t)1 << 24), "%s: %lld sequences out of range", who, (long long)nseq);
-    MI_REQUIRE(offsets || (nseq == 0 ? tokens == 0 : tokens % nseq == 0), "%s: %lld tokens are not %lld sequences of one length", who, (long long)tokens, (long long)nseq);
+    MI_TRY(check_rows(who, tokens, nseq, offsets != nullptr));
     MI_TRY(fill_rows(who, "q", q, tokens, c->heads, c->head_dim, &a->q));
     MI_TRY(fill_rows(who, "k", k, tokens, c->kv_heads, c->head_dim, &a->k));
     MI_TRY(fill_rows(who, "v", v, tokens, c->kv_heads, c->head_dim, &a->v));
@@ -1613,9 +1631,7 @@ static int fill_args(const char* who, mi_ctx* ctx, const mi_attention_config* c,
     a->scale = c->scale;
     a->scale_log2 = c->scale * AT_LOG2E;
     a->scale_inv = 1.0f / c->scale;
-    // one launch: fewer than 2^21 tiles of a head (of at least 64 rows each), 2^31 blocks
-    MI_REQUIRE(tokens / 64 + nseq + 9 < ((int64_t)1 << 21) && (tokens / 64 + nseq + 9) * (int64_t)c->heads < ((int64_t)1 << 31) - 1, "%s: %lld tokens in %lld sequences x %d heads are too many for one call", who, (long long)tokens, (long long)nseq, c->heads);
-    return MI_OK;
+    return check_launch(who, c, tokens, nseq);
 }
 
 extern "C" int mi_attention_dev(mi_ctx* ctx, const mi_attention_config* cfg, int64_t tokens, int64_t nseq, const int32_t* offsets_dev,
@@ -1635,14 +1651,17 @@ extern "C" int mi_attention_dev(mi_ctx* ctx, const mi_attention_config* cfg, int
 extern "C" int mi_attention_backward_workspace(const mi_attention_config* cfg, int64_t tokens, int64_t nseq, int packed, size_t* bytes)
 {
     MI_REQUIRE(cfg && bytes, "mi_attention_backward_workspace: NULL argument");
-    MI_REQUIRE(cfg->heads > 0 && cfg->kv_heads > 0 && cfg->heads % cfg->kv_heads == 0 && cfg->head_dim > 0 && tokens >= 0 && nseq >= 0 && (packed || nseq == 0 || tokens % nseq == 0), "mi_attention_backward_workspace: bad argument");
+    const char* who = "mi_attention_backward_workspace";
+    MI_TRY(check_heads(who, cfg));
+    MI_TRY(check_rows(who, tokens, nseq, packed != 0));
     mi_attn_args a;
     static const int32_t some = 0;
     static const float one = 0.0f;
     if (cfg->num_buckets != 0) {
-        MI_TRY(mi_attn_buckets("mi_attention_backward_workspace", &a, cfg->num_buckets, cfg->max_distance, cfg->bidirectional));
+        MI_TRY(mi_attn_buckets(who, &a, cfg->num_buckets, cfg->max_distance, cfg->bidirectional));
         a.table = &one;
     }
+    MI_TRY(check_launch(who, cfg, tokens, nseq));
     a.offsets = packed ? &some : nullptr;
     a.heads = cfg->heads;
     a.group = cfg->heads / cfg->kv_heads;

@@ -113,3 +113,14 @@ def test_tracing_is_refused(how, backward):
             make_fx(f, pre_dispatch=how.endswith("dispatch"))(q)
     with pytest.raises(ValueError, match="on the GPU"):                        # and afterwards as before
         f(q)
+
+
+def test_workspace_of_calls_that_are_out_of_range():
+    import ctypes
+    from rag_amd import _capi
+    lib, need = _capi.load(), ctypes.c_size_t(7)
+    ok = dict(heads=4, kv_heads=2, head_dim=64, dtype=_capi.DTYPE_BF16, causal=0, zero_tail=0, scale=0.125, num_buckets=0, max_distance=0, bidirectional=0)
+    for change, tokens, nseq in (({}, 1 << 31, 1), ({}, 100, 1 << 24), ({}, 100, (1 << 32) + 2), (dict(heads=65536, kv_heads=1), 100, 1), (dict(head_dim=136), 100, 1),
+                                 (dict(head_dim=60), 100, 1), ({}, (1 << 62), 1), (dict(heads=65535, kv_heads=1), (1 << 31) - 5000, 1)):
+        cfg = _capi.AttentionConfig(*{**ok, **change}.values())
+        assert lib.mi_attention_backward_workspace(cfg, tokens, nseq, 1, ctypes.byref(need)) == -1 and need.value == 7, (change, tokens, nseq)
