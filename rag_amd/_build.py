@@ -34,6 +34,11 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=o
 FILE_FLAGS = {"encoder_ffn3.hip": ["-mllvm", "-amdgpu-spill-vgpr-to-agpr=0"]}
 
 
+def compile_flags(src: str) -> list[str]:
+    """hipcc's flags for one source file of csrc/ (the debug builds under tools/ read them from here)."""
+    return FLAGS + FILE_FLAGS.get(src, [])
+
+
 def _stale(target: str, deps: list[str]) -> bool:
     if not os.path.exists(target):
         return True
@@ -116,7 +121,7 @@ def build_native(force: bool = False, verbose: bool = False) -> str:
         o = os.path.join(OBJDIR, src.replace(".hip", ".o"))
         objs.append(o)
         if force or _stale(o, [s] + hdrs):
-            jobs.append([hipcc, *FLAGS, *FILE_FLAGS.get(src, []), "-c", s, "-o", o])
+            jobs.append([hipcc, *compile_flags(src), "-c", s, "-o", o])
 
     def run(cmd):
         if verbose:
@@ -152,4 +157,9 @@ def build_native(force: bool = False, verbose: bool = False) -> str:
 
 
 if __name__ == "__main__":
-    print(build_native(force="--force" in sys.argv, verbose=True))
+    if sys.argv[1:2] == ["--flags"]:                          # of a source file
+        print(" ".join(compile_flags(sys.argv[2])))
+    elif sys.argv[1:2] == ["--objects"]:                      # of the library, without the named source files'
+        print(" ".join(os.path.join("build", "obj", f.replace(".hip", ".o")) for f in SOURCES if f not in sys.argv[2:]))
+    else:
+        print(build_native(force="--force" in sys.argv, verbose=True))

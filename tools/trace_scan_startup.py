@@ -1,9 +1,8 @@
 """Start-up trace of the MFMA scan: where one workgroup's first units go (200,000 rows x 1 query, L2, F32 index).
 Needs the stamp build of the library, loaded through MI355RAG_LIB:
-  hipcc <FLAGS of rag_amd/_build.py> -DMF_TRACE -DMF_TRACE_U0=0 -c rag_amd/csrc/search_mfma.hip -o tools/_trace/search_mfma.o
-  hipcc --offload-arch=gfx950 -shared -fPIC -o tools/_trace/libtrace.so build/obj/{capi,ingest,search_exact,encoder}.o tools/_trace/search_mfma.o
+  tools/build_trace.sh -DMF_TRACE_U0=0
   MI_MFMA_NS=192 MI355RAG_LIB=tools/_trace/libtrace.so python3 tools/trace_scan_startup.py
-This is how the padding-query compactions (latency section) were found.  Debug tool, not part of the product."""
+This is how the padding-query compactions were found.  Debug tool, not part of the product."""
 import ctypes, sys, os
 import numpy as np
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
