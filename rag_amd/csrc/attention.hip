@@ -1444,11 +1444,17 @@ int mi_launch_attention(hipStream_t st, mi_attn_args a, int dtype)
     return f16 ? launch_fwd<128, true>(st, a) : launch_fwd<128, false>(st, a);
 }
 
-// Shares of a group's query heads in the dK / dV kernel: the fewest that give AT_DKV_BLOCKS blocks (two per CU, four rounds, so
-// that a causal sequence's long first tiles even out), all heads at most.  1 x 8,191 causal, 8 heads on 2 key heads of 128:
-// 130 blocks 1,240 us, 520 blocks 362 us and 12 for joining; 9 prompts up to 2,048, 16 heads on 4: 192 blocks 321, 384 blocks 173 + 10,
-// 768 blocks 123 + 15.
-#define AT_DKV_BLOCKS 2048
+// Shares of a group's query heads in the dK / dV kernel: the fewest that give AT_DKV_BLOCKS blocks (three per CU), all heads at most.  Fewer
+// blocks leave CUs idle, more write and read again 2 x tokens x key heads x head_dim fp32 words each (whole backward pass, us, the shares
+// in brackets; bf16; also measured at 32 heads on 4, at head size 32 and with a bias, with the same outcome):
+//                                              at least 256   512        768        1,024      2,048
+//   8,191 causal, 16 heads on 4 of 128         1,591 (1)      1,066 (2)  1,079 (4)  1,080 (4)  1,079 (4)
+//   9 prompts up to 2,048, the same heads        252 (2)        208 (4)    208 (4)    208 (4)    208 (4)
+//   60 x 300, the same heads                     309 (1)        310 (1)    310 (1)    395 (2)    455 (4)
+//   60 x 300, 16 heads on 2 of 64                157 (1)        153 (2)    153 (2)    164 (4)    189 (8)
+//   300 x 40, 16 heads on 2 of 32                 53 (1)         54 (1)     53 (1)     63 (2)     65 (4)
+//   8,191 causal, 32 heads on 4 of 64          1,306 (1)      1,055 (2)  1,041 (4)  1,038 (4)  1,010 (8)
+#define AT_DKV_BLOCKS 768
 static int at_dkv_splits(const mi_attn_args& a)
 {
     const int64_t blocks = (int64_t)(a.heads / a.group) * (a.tokens / 128 + a.nseq);

@@ -51,12 +51,13 @@ def test_one_token_of_each_sequence_as_a_view(at):
     assert torch.equal(a[0], z["v"].repeat_interleave(2, 2))
 
 
-@pytest.mark.parametrize("H,Hk,repeats,splits", [(8, 4, 44, 1), (16, 4, 25, 2), (32, 16, 12, 1)])
+@pytest.mark.parametrize("H,Hk,repeats,splits", [(8, 4, 44, 1), (8, 4, 17, 1), (16, 4, 12, 2), (16, 4, 9, 2), (32, 16, 12, 1)])
 @pytest.mark.parametrize("table", [0, 32])
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("D,dtype", [(32, "bf16"), (64, "fp16"), (128, "bf16"), (128, "fp16")])
 def test_blocks_that_walk_several_query_heads(D, dtype, causal, table, H, Hk, repeats, splits):
-    """Large batches of grouped heads: a dK / dV block takes group / splits > 1 query heads one after another.  The batch repeats a
+    """Large batches of grouped heads: a dK / dV block takes group / splits > 1 query heads one after another, up to head size 64 with its
+    rows split over two waves (17 and 9 repeats: fewer than 1,024 blocks) or not.  The batch repeats a
     pattern of sequences, so that the 64-bit form is worked out for one: a repeat's results are the first's, bit for bit, and the
     table's gradient is the sum of the repeats'."""
     import torch
