@@ -58,7 +58,7 @@ def _rows(name: str, t, shape, dtype, device) -> AttentionRows:
 
 
 def _own_rows(t, heads, hd) -> AttentionRows:
-    """... of a contiguous tensor made here: nothing to check."""
+    """... of a contiguous tensor made here, or q itself: nothing to check."""
     return AttentionRows(t.data_ptr(), heads * hd, hd)
 
 
@@ -190,11 +190,13 @@ def packed_attention(q, k, v, offsets=None, *, causal: bool = False, scale: Opti
 def _forward(q, k, v, offsets, causal, scale, key_mask, bias_table, max_distance, bidirectional, with_lse):
     cfg, tokens, nseq, off, mask, table = _setup(q, k, v, offsets, causal, scale, key_mask, bias_table, max_distance, bidirectional)
     z, zk, dtype, device = q.shape, k.shape, q.dtype, q.device
-    out = _like(q)
+    own = q.is_contiguous()
+    out = _empty_like(q) if own else _like(q)
     lse = q.new_empty((z[-2], tokens), dtype=_F32) if with_lse else None
-    _capi.check(_capi.load().mi_attention_dev(_capi.get_ctx(device.index), cfg, tokens, nseq, off, mask, _rows("q", q, z, dtype, device),
-                                              _rows("k", k, zk, dtype, device), _rows("v", v, zk, dtype, device), table,
-                                              _own_rows(out, z[-2], z[-1]), lse.data_ptr() if with_lse else None, _capi.stream_arg(device)))
+    _capi.check(_capi.load().mi_attention_dev(_capi.get_ctx(device.index), cfg, tokens, nseq, off, mask,
+                                              _own_rows(q, z[-2], z[-1]) if own else _rows("q", q, z, dtype, device),
+                                              _rows("k", k, zk, dtype, device), _rows("v", v, zk, dtype, device), table, _own_rows(out, z[-2], z[-1]),
+                                              lse.data_ptr() if with_lse else None, _capi.stream_arg(device)))
     return out, lse
 
 
@@ -249,8 +251,8 @@ def packed_attention_backward(dout, q, k, v, out, lse, offsets=None, *, causal: 
     heads = z[-2]
     if lse.dtype != _F32 or tuple(lse.shape) != (heads, tokens) or not lse.is_contiguous() or lse.device != device:
         raise ValueError(f"packed_attention_backward: lse must be the contiguous float32 [{heads}][{tokens}] tensor of the forward pass")
-    rows = (_rows("q", q, z, dtype, device), _rows("k", k, zk, dtype, device), _rows("v", v, zk, dtype, device), _rows("out", out, z, dtype, device),
-            _rows("dout", dout, z, dtype, device))
+    rows = (_own_rows(q, heads, z[-1]) if q.is_contiguous() else _rows("q", q, z, dtype, device), _rows("k", k, zk, dtype, device),
+            _rows("v", v, zk, dtype, device), _rows("out", out, z, dtype, device), _rows("dout", dout, z, dtype, device))
     dq, dk, dv = _like(q), _like(k), _like(v)
     dtable = _like(bias_table) if bias_table is not None else None
     work = q.new_empty(_workspace(heads, zk[-2], z[-1], cfg.num_buckets, cfg.max_distance, cfg.bidirectional, tokens, nseq, offsets is not None), dtype=_F32)

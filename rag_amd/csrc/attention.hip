@@ -1413,6 +1413,8 @@ static int at_lds(size_t bytes)
 // 64, bias) 76 -> 56 us, 520 (8,191, 8 heads of 128) 178 -> 160 us; 1,500 blocks (prompts up to 2,039, 32 heads of 128) 75 ->
 // 87 us, 2,048 (16,384, 16 heads of 128) 1,066 -> 1,243 us, 8,900 (chunks up to 256, 12 heads of 32) 67 -> 83 us.  Backward: 256
 // blocks (a document of 4,000, 8 heads of 64, bias) dQ 98 -> 73 us, dK / dV 99 -> 68 us; 512 (8,191, 8 heads of 128) dQ 255 -> 228 us.
+// (Blocks are counted, not their work: a batch of short sequences is split like one document, and with up to 32 keys the second wave of a
+// row has nothing to do.)
 static bool at_few(const mi_attn_args& a, int heads) { return (int64_t)heads * (a.tokens / 128 + a.nseq) < 1024; }
 
 template <int DP, bool F16, bool BIAS, int KS>
@@ -1473,6 +1475,9 @@ size_t mi_attn_backward_bytes(const mi_attn_args& a)
     return delta + join + (a.table ? (size_t)(a.heads * tiles) * MI_ATTN_MAX_BUCKETS * 4 : 0);
 }
 
+// With a bias the LDS of a dQ block grows by 40 bytes for each distance of `reach` (the bias and the waves' sums over r): two blocks a CU up to
+// reach 466 at head size 32, 262 at 64 (210 with two waves to a row), one beyond, and at 128 (48 buckets, 100 x 512 rows of 12 heads of 64: reach
+// 244 385 us, reach 288 675 us; 12 of 32: reach 374 331 us, reach 707 697 us).
 template <int DP, bool F16, bool BIAS, int KS>
 static int launch_dq(hipStream_t st, mi_attn_args& a)
 {
