@@ -459,7 +459,8 @@ class MI355Embeddings:
     listed GPU in this one process and splits every bulk call over them -- pure data parallel, no collective, input
     order kept (BASELINE config 3 from the single process advanced_rag.py is); `slab_texts` is the number of texts
     tokenised per step of the host pipeline below.  A model whose directory holds a relative position bias
-    (load_local_position_bias) runs with it; model_kwargs={"causal": True} runs a model trained with causal attention."""
+    (load_local_position_bias) runs with it, with buckets for both directions; model_kwargs={"causal": True} runs a model trained with causal
+    attention (one with one-sided buckets: set_attention on each of its `encoders`)."""
 
     def __init__(self, model_name: str, cache_folder: Optional[str] = None,
                  model_kwargs: Optional[Dict[str, Any]] = None, encode_kwargs: Optional[Dict[str, Any]] = None,
