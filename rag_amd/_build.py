@@ -1,7 +1,6 @@
 """Builds rag_amd/lib/libmi355rag.so from rag_amd/csrc/*.hip with hipcc for gfx950.
 
-hipcc cross-compiles without a GPU, so this runs in the build container; the resulting .so
-travels to the GPU box with the tree (it is git-ignored, not gpurun-ignored).
+hipcc cross-compiles without a GPU, so this runs where there is none; the .so is git-ignored and travels with the tree.
 """
 from __future__ import annotations
 
@@ -85,7 +84,7 @@ def audit_ffn3(workdir: str | None = None, extra_flags=()) -> None:
 # Files whose kernels (names containing the substring) must compile without a single spilled register or byte of scratch:
 # the scan kernels sit at 250-256 VGPRs with two waves per SIMD, and one more live value makes hipcc spill ~200 registers --
 # the kernel stays correct and gets 2.3 x slower at 512 queries (a scratch reload in the loop waits for vmcnt(0), which drains
-# the LDS-DMA prefetch).  Measured the hard way in round 3.
+# the LDS-DMA prefetch).
 NO_SPILL = {"search_mfma.hip": "mfma_scan_kernel", "encoder_qkv_attn.hip": "qkv_attn_kernel"}
 
 
